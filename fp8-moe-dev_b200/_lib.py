@@ -37,9 +37,13 @@ EXPORTS = [
     "moe_fp8_b200_exchange_regions", "moe_fp8_b200_copy_rows_h2d",
     "moe_fp8_b200_invalidate_weights", "moe_fp8_b200_copy_device", "moe_fp8_b200_signal_peers",
     "moe_fp8_b200_wait_peers", "moe_fp8_b200_create_shaped", "moe_fp8_b200_workspace_bytes_shaped",
-    "moe_fp8_b200_get_shape", "moe_fp8_b200_host_path",
+    "moe_fp8_b200_get_shape", "moe_fp8_b200_host_path", "moe_fp8_b200_plan_rows", "moe_fp8_b200_sort_tokens",
+    "moe_fp8_b200_dispatch_rows", "moe_fp8_b200_sort_and_dispatch", "moe_fp8_b200_combine_rows",
+    "moe_fp8_b200_combine_rows_backward",
 ]
 NOALLOC_MAX_TOKENS = 4096
+BF16, FP16, FP32 = 0, 1, 2
+PLAN_MAX_TOP_K, PLAN_MAX_EXPERTS = 16, 1024
 
 
 class Args(C.Structure):
@@ -68,6 +72,13 @@ class Unfinalized(C.Structure):
     """moe_fp8_b200_unfinalized"""
     _fields_ = [("y", C.c_void_p), ("expert_offset", C.c_void_p), ("pair_count", C.c_void_p),
                 ("pair_code", C.c_void_p), ("pair_weight", C.c_void_p), ("row_capacity", C.c_int32)]
+
+
+class Plan(C.Structure):
+    """moe_fp8_b200_plan"""
+    _fields_ = [("num_tokens", C.c_int32), ("top_k", C.c_int32), ("num_experts", C.c_int32), ("align", C.c_int32),
+                ("pair_row", C.c_void_p), ("row_pair", C.c_void_p), ("expert_offset", C.c_void_p),
+                ("expert_count", C.c_void_p)]
 
 
 _lib = None
@@ -152,6 +163,18 @@ def load() -> C.CDLL:
     lib.moe_fp8_b200_stage_times.argtypes = [H, C.POINTER(C.c_float), C.POINTER(C.c_int)]
     lib.moe_fp8_b200_reference_policy.restype = C.c_int
     lib.moe_fp8_b200_reference_policy.argtypes = [C.c_int, C.POINTER(C.c_int32), C.POINTER(C.c_float)]
+    P, PLAN, I64, ERR = C.c_void_p, C.POINTER(Plan), C.c_int64, (C.c_void_p, C.c_char_p, C.c_size_t)
+    lib.moe_fp8_b200_plan_rows.restype = I64
+    lib.moe_fp8_b200_plan_rows.argtypes = [C.c_int, C.c_int, C.c_int, C.c_int]
+    for name, argtypes in dict(
+            sort_tokens=(P, C.c_int, I64, PLAN),
+            dispatch_rows=(P, I64, P, I64, C.c_int, C.c_int, PLAN, C.c_int),
+            sort_and_dispatch=(P, C.c_int, I64, P, I64, P, I64, C.c_int, C.c_int, PLAN, C.c_int),
+            combine_rows=(P, I64, P, P, I64, C.c_int, C.c_int, PLAN),
+            combine_rows_backward=(P, I64, P, I64, P, P, I64, P, C.c_int, C.c_int, PLAN, C.c_int)).items():
+        fn = getattr(lib, "moe_fp8_b200_" + name)
+        fn.restype = C.c_int
+        fn.argtypes = [*argtypes, *ERR]
     _lib = lib
     return lib
 

@@ -1,0 +1,299 @@
+"""The operators around a caller's own experts, on top of the C ABI: tokens sorted by expert and copied to packed rows,
+the experts' rows back at their tokens with the routing weights applied, and the gradients of both.
+
+    plan = sort_tokens(topk_idx, num_experts)              # which packed row every (token, expert) pair has
+    rows = dispatch(x, plan)                               # [plan.capacity, hidden], grouped by expert
+    y = ...                                                # the experts' results, row by row
+    out = combine(y, topk_weights, plan)                   # [T, hidden]
+
+`sort_and_dispatch` is the first two in one call.  `dispatch` and `combine` take part in autograd; `dispatch_backward`
+and `combine_backward` are their gradients as plain calls.  Results go to the tensors passed for them, or to new ones.
+Everything runs on the current stream of the tensors' device and returns without synchronising.  The counterparts
+inside the reference's layer are kernel/moe_fp8.cu:1064-1115 (permute) and :2254-2323 (combine).
+"""
+from __future__ import annotations
+
+import ctypes as C
+from typing import Optional, Tuple
+
+import torch
+
+from . import _lib
+from .op import MoeError
+
+_ROW_TYPES = {torch.bfloat16: _lib.BF16, torch.float16: _lib.FP16, torch.float32: _lib.FP32}
+_ID_BITS = {torch.int32: 32, torch.int64: 64}
+_raw_stream = torch._C._cuda_getCurrentRawStream
+_ERR_BYTES = 256
+
+
+def _call(fn, device, *args):
+    """fn(*args, stream, err, err_len) with the tensors' device current."""
+    err = C.create_string_buffer(_ERR_BYTES)
+    index = device.index
+    if index == torch.cuda.current_device():
+        rc = fn(*args, _raw_stream(index), err, _ERR_BYTES)
+    else:
+        with torch.cuda.device(index):
+            rc = fn(*args, _raw_stream(index), err, _ERR_BYTES)
+    if rc != _lib.OK:
+        raise MoeError(rc, err.value.decode())
+
+
+def _on_gpu(name, t):
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor")
+    if not t.is_cuda:
+        raise ValueError(f"{name} must live on a CUDA device, got {t.device}")
+    return t.device
+
+
+def _packed(name, t, dtype, shape, device):
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor")
+    if t.dtype != dtype:
+        raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
+    if t.shape != shape:
+        raise ValueError(f"{name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
+    if not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous")
+    if t.device != device:
+        raise ValueError(f"{name} must live on {device}, got {t.device}")
+    return t.data_ptr()
+
+
+def _matrix(name, t, rows, columns, dtype, device):
+    """A [rows, columns] matrix whose rows are contiguous, at any stride: its address and stride."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor")
+    if t.dtype != dtype:
+        raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
+    if t.dim() != 2 or t.shape[0] != rows or t.shape[1] != columns:
+        raise ValueError(f"{name} must have shape ({rows}, {columns}), got {tuple(t.shape)}")
+    stride, column = t.stride()
+    if column != 1 and columns > 1:
+        raise ValueError(f"{name}: the elements of a row must be contiguous")
+    if t.device != device:
+        raise ValueError(f"{name} must live on {device}, got {t.device}")
+    return t.data_ptr(), stride
+
+
+def _row_type(name, t):
+    if t.dtype not in _ROW_TYPES:
+        raise TypeError(f"{name} must be bfloat16, float16 or float32, got {t.dtype}")
+    if t.dim() != 2 or t.shape[1] < 1:
+        raise ValueError(f"{name} must be a matrix with at least one column, got shape {tuple(t.shape)}")
+    return _ROW_TYPES[t.dtype]
+
+
+def plan_rows(num_tokens: int, top_k: int, num_experts: int, align: int = 1) -> int:
+    """Rows that any choice of experts fits into: what `rows` of a dispatch must hold."""
+    rows = _lib.load().moe_fp8_b200_plan_rows(int(num_tokens), int(top_k), int(num_experts), int(align))
+    if rows < 0:
+        raise ValueError(f"no plan for {num_tokens} tokens, top_k {top_k} (1 .. {_lib.PLAN_MAX_TOP_K}), {num_experts} experts "
+                         f"(1 .. {_lib.PLAN_MAX_EXPERTS}), align {align} (1 .. 1024)")
+    return int(rows)
+
+
+class ExpertPlan:
+    """Which packed row every (token, expert) pair has.  Rows are ordered by expert, within an expert by pair
+    t * top_k + k; each expert starts a multiple of `align` rows after the one before it.
+
+      pair_row       int32 [T, top_k]    row of each pair, -1 where its expert is not one of this plan's
+      row_pair       int32 [capacity]    pair of each row, -1 in an expert's padding and behind the last expert
+      expert_offset  int32 [E + 1]       first row of each expert, and the end of the last one
+      expert_count   int32 [E]           pairs of each expert
+
+    Made by sort_tokens, or from four tensors of one's own (to be filled, or filled elsewhere)."""
+    __slots__ = ("pair_row", "row_pair", "expert_offset", "expert_count", "align", "num_tokens", "top_k", "num_experts",
+                 "capacity", "device", "_c")
+
+    def __init__(self, pair_row, row_pair, expert_offset, expert_count, *, align: int = 1):
+        device = _on_gpu("pair_row", pair_row)
+        if pair_row.dim() != 2:
+            raise ValueError(f"pair_row must have shape (tokens, top_k), got {tuple(pair_row.shape)}")
+        T, K = pair_row.shape
+        E = expert_count.shape[0] if isinstance(expert_count, torch.Tensor) and expert_count.dim() == 1 else 0
+        self.num_tokens, self.top_k, self.num_experts, self.align = T, K, E, int(align)
+        self.capacity = plan_rows(T, K, E, self.align)
+        self.pair_row, self.row_pair, self.expert_offset, self.expert_count = pair_row, row_pair, expert_offset, expert_count
+        self.device = device
+        self._c = C.byref(_lib.Plan(T, K, E, self.align, _packed("pair_row", pair_row, torch.int32, (T, K), device),
+                                    _packed("row_pair", row_pair, torch.int32, (self.capacity,), device),
+                                    _packed("expert_offset", expert_offset, torch.int32, (E + 1,), device),
+                                    _packed("expert_count", expert_count, torch.int32, (E,), device)))
+
+    @classmethod
+    def empty(cls, num_tokens: int, top_k: int, num_experts: int, align: int = 1, device="cuda") -> "ExpertPlan":
+        """A plan to be filled."""
+        def ints(*shape):
+            return torch.empty(shape, dtype=torch.int32, device=device)
+        return cls(ints(num_tokens, top_k), ints(plan_rows(num_tokens, top_k, num_experts, align)), ints(num_experts + 1),
+                   ints(num_experts), align=align)
+
+
+def _check_plan(plan):
+    if not isinstance(plan, ExpertPlan):
+        raise TypeError("plan must be an ExpertPlan")
+    return plan.device
+
+
+def _ids(topk_idx, num_experts, align, plan):
+    """The plan to fill for these ids."""
+    device = _on_gpu("topk_idx", topk_idx)
+    if topk_idx.dtype not in _ID_BITS:
+        raise TypeError(f"topk_idx must be int32 or int64, got {topk_idx.dtype}")
+    if topk_idx.dim() != 2:
+        raise ValueError(f"topk_idx must have shape (tokens, top_k), got {tuple(topk_idx.shape)}")
+    if not topk_idx.is_contiguous():
+        raise ValueError("topk_idx must be contiguous")
+    T, K = topk_idx.shape
+    if plan is None:
+        return ExpertPlan.empty(T, K, int(num_experts), int(align), device)
+    if _check_plan(plan) != device:
+        raise ValueError(f"plan must live on {device}, got {plan.device}")
+    if (plan.num_tokens, plan.top_k, plan.num_experts, plan.align) != (T, K, num_experts, align):
+        raise ValueError(f"plan is for {plan.num_tokens} tokens, top_k {plan.top_k}, {plan.num_experts} experts, align {plan.align}; "
+                         f"the call has {T}, {K}, {num_experts}, {align}")
+    return plan
+
+
+def sort_tokens(topk_idx, num_experts: int, *, first_expert: int = 0, align: int = 1,
+                plan: Optional[ExpertPlan] = None) -> ExpertPlan:
+    """Sorts the (token, expert) pairs of topk_idx [T, top_k] (int32 or int64) by expert.  The plan's experts are
+    [first_expert, first_expert + num_experts); pairs of other experts (an id of -1, another GPU's expert) have no row."""
+    plan = _ids(topk_idx, num_experts, align, plan)
+    _call(_lib.load().moe_fp8_b200_sort_tokens, plan.device, topk_idx.data_ptr(), _ID_BITS[topk_idx.dtype], first_expert,
+          plan._c)
+    return plan
+
+
+def _rows_for(x, plan, rows):
+    """Arguments of the copy to packed rows: the matrix, and its C arguments."""
+    kind = _row_type("x", x)
+    H = x.shape[1]
+    xp, xs = _matrix("x", x, plan.num_tokens, H, x.dtype, plan.device)
+    fresh = rows is None
+    if fresh:
+        rows = torch.empty((plan.capacity, H), dtype=x.dtype, device=plan.device)
+    rp, rs = _matrix("rows", rows, plan.capacity, H, x.dtype, plan.device)
+    return rows, (xp, xs, rp, rs, kind, H, plan._c, int(fresh))
+
+
+def _wants_grad(*tensors):
+    return torch.is_grad_enabled() and any(t.requires_grad for t in tensors)
+
+
+def dispatch(x, plan: ExpertPlan, rows=None):
+    """rows[r] = x[token of row r], zeros in the experts' padding; rows behind the last expert stay as they were (in
+    a new matrix: zeros).  x [T, hidden], rows [plan.capacity, hidden]: bfloat16, float16 or float32, any row stride.
+    Differentiable in x (not together with `rows`)."""
+    _check_plan(plan)
+    if _wants_grad(x):
+        if rows is not None:
+            raise ValueError("rows cannot be given where x requires a gradient")
+        return _Dispatch.apply(x, plan)
+    rows, args = _rows_for(x, plan, rows)
+    _call(_lib.load().moe_fp8_b200_dispatch_rows, plan.device, *args)
+    return rows
+
+
+def sort_and_dispatch(x, topk_idx, num_experts: int, *, first_expert: int = 0, align: int = 1,
+                      plan: Optional[ExpertPlan] = None, rows=None) -> Tuple[torch.Tensor, ExpertPlan]:
+    """sort_tokens and dispatch in one call: (rows, plan)."""
+    plan = _ids(topk_idx, num_experts, align, plan)
+    if _wants_grad(x):
+        return dispatch(x, sort_tokens(topk_idx, num_experts, first_expert=first_expert, align=align, plan=plan), rows), plan
+    rows, args = _rows_for(x, plan, rows)
+    _call(_lib.load().moe_fp8_b200_sort_and_dispatch, plan.device, topk_idx.data_ptr(), _ID_BITS[topk_idx.dtype], first_expert,
+          *args)
+    return rows, plan
+
+
+def _combine(y, weights, plan, out):
+    kind = _row_type("y", y)
+    H = y.shape[1]
+    yp, ys = _matrix("y", y, plan.capacity, H, y.dtype, plan.device)
+    wp = None if weights is None else _packed("weights", weights, torch.float32, (plan.num_tokens, plan.top_k), plan.device)
+    if out is None:
+        out = torch.empty((plan.num_tokens, H), dtype=y.dtype, device=plan.device)
+    op, os = _matrix("out", out, plan.num_tokens, H, y.dtype, plan.device)
+    _call(_lib.load().moe_fp8_b200_combine_rows, plan.device, yp, ys, wp, op, os, kind, H, plan._c)
+    return out
+
+
+def combine(y, weights, plan: ExpertPlan, out=None):
+    """out[t] = sum over token t's rows of weights[t, k] * y[row], in fp32 and pair order, rounded once; zeros for a token
+    without rows.  y [plan.capacity, hidden], weights fp32 [T, top_k].  Padding and unused rows of y are not read.
+    Differentiable in y and weights (not together with `out`)."""
+    _check_plan(plan)
+    if _wants_grad(y, weights):
+        if out is not None:
+            raise ValueError("out cannot be given where y or weights require a gradient")
+        return _Combine.apply(y, weights, plan)
+    return _combine(y, weights, plan, out)
+
+
+def dispatch_backward(grad_rows, plan: ExpertPlan, out=None):
+    """Gradient of dispatch's x from that of its rows: out[t] = the sum of token t's rows."""
+    _check_plan(plan)
+    return _combine(grad_rows, None, plan, out)
+
+
+def combine_backward(grad_out, y, weights, plan: ExpertPlan, grad_y=None, grad_weights=None, *, need_y: bool = True,
+                     need_weights: bool = True):
+    """Gradients of combine: (grad_y [plan.capacity, hidden], grad_weights fp32 [T, top_k]).  grad_y is zero in the
+    experts' padding and untouched behind the last expert (in a new matrix: zero there too); grad_weights is 0 where a pair has no row.  A gradient that is
+    not needed is None."""
+    _check_plan(plan)
+    kind = _row_type("grad_out", grad_out)
+    H, dtype, device = grad_out.shape[1], grad_out.dtype, plan.device
+    gp, gs = _matrix("grad_out", grad_out, plan.num_tokens, H, dtype, device)
+    yp, ys = _matrix("y", y, plan.capacity, H, dtype, device)
+    wp = _packed("weights", weights, torch.float32, (plan.num_tokens, plan.top_k), device)
+    dp, ds, dwp = None, 0, None
+    fresh = grad_y is None
+    if need_y:
+        if fresh:
+            grad_y = torch.empty((plan.capacity, H), dtype=dtype, device=device)
+        dp, ds = _matrix("grad_y", grad_y, plan.capacity, H, dtype, device)
+    if need_weights:
+        if grad_weights is None:
+            grad_weights = torch.empty((plan.num_tokens, plan.top_k), dtype=torch.float32, device=device)
+        dwp = _packed("grad_weights", grad_weights, torch.float32, (plan.num_tokens, plan.top_k), device)
+    _call(_lib.load().moe_fp8_b200_combine_rows_backward, device, gp, gs, yp, ys, wp, dp, ds, dwp, kind, H, plan._c,
+          int(fresh))
+    return grad_y if need_y else None, grad_weights if need_weights else None
+
+
+def _plain_rows(grad):
+    # autograd may hand in a broadcast gradient (of a sum, say)
+    return grad if grad.stride(1) == 1 else grad.contiguous()
+
+
+class _Dispatch(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, plan):
+        ctx.plan = plan
+        return dispatch(x.detach(), plan)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad_rows):
+        return dispatch_backward(_plain_rows(grad_rows), ctx.plan), None
+
+
+class _Combine(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, y, weights, plan):
+        ctx.plan = plan
+        ctx.save_for_backward(y, weights)
+        return _combine(y.detach(), weights.detach(), plan, None)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad_out):
+        y, weights = ctx.saved_tensors
+        grad_y, grad_weights = combine_backward(_plain_rows(grad_out), y, weights, ctx.plan,
+                                                need_y=ctx.needs_input_grad[0], need_weights=ctx.needs_input_grad[1])
+        return grad_y, grad_weights, None

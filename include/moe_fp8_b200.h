@@ -420,6 +420,74 @@ MOE_FP8_B200_API int moe_fp8_b200_route_noalloc(const float* routing_logits, con
                                                 float* topk_weight_out, int32_t* expert_count_out, void* stream,
                                                 char* err, size_t err_len);
 
+/* ---- tokens sorted by expert and back -----------------------------------------------------
+ * The movement either side of a caller's own experts, for any row type and expert count, with its gradients.  The
+ * reference has it only inside its layer, for its e4m3 rows (kernel/moe_fp8.cu:1064-1115, 2254-2323).  These functions
+ * need no handle and allocate nothing: they work on the CURRENT CUDA device, refuse tensors of another one, enqueue on
+ * `stream` and return without synchronising; they may be captured into a graph.  err / err_len: optional buffer
+ * for an error message (may be NULL / 0).
+ *
+ * A plan says which packed row every (token, expert) pair has.  Pair t * top_k + k belongs to the local expert
+ * e = topk_idx[t, k] - first_expert; pairs with e outside [0, num_experts) have no row.  Rows are ordered by expert and
+ * within an expert by pair.  Expert e owns rows [expert_offset[e], expert_offset[e] + expert_count[e]); expert_offset[e + 1]
+ * is its end rounded up so that the next expert starts a multiple of `align` rows further (128: the 128-row tiles of a
+ * grouped GEMM never hold two experts).  The rows between are its padding, the rows behind
+ * expert_offset[num_experts] are unused.  The caller owns the four arrays. */
+typedef struct moe_fp8_b200_plan {
+    int32_t num_tokens;     /* T, 0 .. */
+    int32_t top_k;          /* 1 .. MOE_FP8_B200_PLAN_MAX_TOP_K */
+    int32_t num_experts;    /* E, 1 .. MOE_FP8_B200_PLAN_MAX_EXPERTS */
+    int32_t align;          /* 1 .. 1024 */
+    int32_t* pair_row;      /* [T, top_k]  row of each pair, -1 = none */
+    int32_t* row_pair;      /* [moe_fp8_b200_plan_rows(...)]  pair of each row, -1 = padding or unused */
+    int32_t* expert_offset; /* [E + 1] */
+    int32_t* expert_count;  /* [E] */
+} moe_fp8_b200_plan;
+#define MOE_FP8_B200_PLAN_MAX_TOP_K 16
+#define MOE_FP8_B200_PLAN_MAX_EXPERTS 1024
+
+/* Row types. */
+enum { MOE_FP8_B200_BF16 = 0, MOE_FP8_B200_FP16 = 1, MOE_FP8_B200_FP32 = 2 };
+
+/* Rows that any choice of experts fits into: T * top_k + min(E, T * top_k) * (align - 1), rounded up to a multiple of
+ * align; 0 for T == 0, -1 where the sizes are refused (among them a result of 2^31 or more).  Host only. */
+MOE_FP8_B200_API int64_t moe_fp8_b200_plan_rows(int num_tokens, int top_k, int num_experts, int align);
+
+/* Fills the plan from expert ids [T, top_k] of id_bits = 32 or 64 bits each.  Any ids are safe; the same expert twice
+ * in a token gives two rows. */
+MOE_FP8_B200_API int moe_fp8_b200_sort_tokens(const void* topk_idx, int id_bits, int64_t first_expert,
+                                              const moe_fp8_b200_plan* plan, void* stream, char* err, size_t err_len);
+
+/* rows[r, :] = x[row_pair[r] / top_k, :] for the rows that have a pair, zeros for the padding; unused rows are left as
+ * they were, or zeroed too with zero_unused != 0.  x is [T, hidden] with `x_stride` elements from row to row, rows [plan_rows, hidden] with `rows_stride`.
+ * Rows whose addresses and length are multiples of 16 bytes move in 16-byte pieces, others element by element.
+ * The plan must be one that moe_fp8_b200_sort_tokens filled for these sizes. */
+MOE_FP8_B200_API int moe_fp8_b200_dispatch_rows(const void* x, int64_t x_stride, void* rows, int64_t rows_stride, int dtype,
+                                                int hidden, const moe_fp8_b200_plan* plan, int zero_unused, void* stream,
+                                                char* err, size_t err_len);
+
+/* Both of the above in one call. */
+MOE_FP8_B200_API int moe_fp8_b200_sort_and_dispatch(const void* topk_idx, int id_bits, int64_t first_expert, const void* x,
+                                                    int64_t x_stride, void* rows, int64_t rows_stride, int dtype, int hidden,
+                                                    const moe_fp8_b200_plan* plan, int zero_unused, void* stream, char* err,
+                                                    size_t err_len);
+
+/* out[t, :] = sum over the token's rows of weights[t, k] * y[pair_row[t, k], :], accumulated with fp32 FMAs in pair order
+ * and rounded once; zeros for a token without rows.  weights fp32 [T, top_k]; NULL = all 1, which is the gradient of
+ * moe_fp8_b200_dispatch_rows with y = the gradient of its rows. */
+MOE_FP8_B200_API int moe_fp8_b200_combine_rows(const void* y, int64_t y_stride, const float* weights, void* out,
+                                               int64_t out_stride, int dtype, int hidden, const moe_fp8_b200_plan* plan,
+                                               void* stream, char* err, size_t err_len);
+
+/* The gradients of moe_fp8_b200_combine_rows: grad_y[r, :] = weights[pair] * grad_out[token, :] (padding rows zero,
+ * unused rows left as they were, or zeroed too with zero_unused != 0) and grad_weights[t, k] = <grad_out[t, :], y[pair_row[t, k], :]>, summed in fp32 in a fixed
+ * order (0 for a pair without a row).  Either may be NULL if it is not wanted; y may be NULL with grad_weights. */
+MOE_FP8_B200_API int moe_fp8_b200_combine_rows_backward(const void* grad_out, int64_t grad_out_stride, const void* y,
+                                                        int64_t y_stride, const float* weights, void* grad_y,
+                                                        int64_t grad_y_stride, float* grad_weights, int dtype, int hidden,
+                                                        const moe_fp8_b200_plan* plan, int zero_unused, void* stream,
+                                                        char* err, size_t err_len);
+
 #ifdef __cplusplus
 }
 #endif
