@@ -3,5 +3,5 @@ on top of the C ABI in include/moe_fp8_b200.h.  Import name: fp8_moe_dev_b200 (t
 name holds a hyphen, so the repo root's __graft_entry__.load_package() registers it)."""
 from . import _lib  # noqa: F401
 from .op import MoeError, MoeLayer, expert_loads, run  # noqa: F401
-from .experts import (ExpertPlan, combine, combine_backward, dispatch, dispatch_backward, plan_rows,  # noqa: F401
-                      sort_and_dispatch, sort_tokens)
+from .experts import (ExpertPlan, combine, combine_backward, dispatch, dispatch_backward, matvec_w4,  # noqa: F401
+                      plan_rows, sort_and_dispatch, sort_tokens)

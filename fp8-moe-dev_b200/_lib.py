@@ -39,7 +39,7 @@ EXPORTS = [
     "moe_fp8_b200_wait_peers", "moe_fp8_b200_create_shaped", "moe_fp8_b200_workspace_bytes_shaped",
     "moe_fp8_b200_get_shape", "moe_fp8_b200_host_path", "moe_fp8_b200_plan_rows", "moe_fp8_b200_sort_tokens",
     "moe_fp8_b200_dispatch_rows", "moe_fp8_b200_sort_and_dispatch", "moe_fp8_b200_combine_rows",
-    "moe_fp8_b200_combine_rows_backward",
+    "moe_fp8_b200_combine_rows_backward", "moe_fp8_b200_matvec_w4",
 ]
 NOALLOC_MAX_TOKENS = 4096
 BF16, FP16, FP32 = 0, 1, 2
@@ -79,6 +79,12 @@ class Plan(C.Structure):
     _fields_ = [("num_tokens", C.c_int32), ("top_k", C.c_int32), ("num_experts", C.c_int32), ("align", C.c_int32),
                 ("pair_row", C.c_void_p), ("row_pair", C.c_void_p), ("expert_offset", C.c_void_p),
                 ("expert_count", C.c_void_p)]
+
+
+class W4(C.Structure):
+    """moe_fp8_b200_w4"""
+    _fields_ = [("codes", C.c_void_p), ("scales", C.c_void_p), ("zeros", C.c_void_p), ("num_experts", C.c_int32),
+                ("n", C.c_int32), ("k", C.c_int32), ("group", C.c_int32)]
 
 
 _lib = None
@@ -171,7 +177,8 @@ def load() -> C.CDLL:
             dispatch_rows=(P, I64, P, I64, C.c_int, C.c_int, PLAN, C.c_int),
             sort_and_dispatch=(P, C.c_int, I64, P, I64, P, I64, C.c_int, C.c_int, PLAN, C.c_int),
             combine_rows=(P, I64, P, P, I64, C.c_int, C.c_int, PLAN),
-            combine_rows_backward=(P, I64, P, I64, P, P, I64, P, C.c_int, C.c_int, PLAN, C.c_int)).items():
+            combine_rows_backward=(P, I64, P, I64, P, P, I64, P, C.c_int, C.c_int, PLAN, C.c_int),
+            matvec_w4=(P, I64, C.c_int, C.POINTER(W4), C.c_int, P, I64, C.c_int, PLAN, C.c_int)).items():
         fn = getattr(lib, "moe_fp8_b200_" + name)
         fn.restype = C.c_int
         fn.argtypes = [*argtypes, *ERR]

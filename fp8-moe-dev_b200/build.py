@@ -27,7 +27,7 @@ NVCC_FLAGS = [
     "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=hidden",
 ]
 CU_SOURCES = ["routing.cu", "gemm.cu", "expert_gemms.cu", "moe_api.cu", "noalloc.cu", "quantize.cu", "decode.cu",
-              "expert_rows.cu"]
+              "expert_rows.cu", "matvec4.cu"]
 
 
 def _nvcc() -> str:

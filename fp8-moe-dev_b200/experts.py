@@ -266,6 +266,55 @@ def combine_backward(grad_out, y, weights, plan: ExpertPlan, grad_y=None, grad_w
     return grad_y if need_y else None, grad_weights if need_weights else None
 
 
+def matvec_w4(x, codes, scales, *, zeros=None, plan: Optional[ExpertPlan] = None, by_token: bool = False, gated: bool = False,
+              out=None):
+    """Products of a few rows with 4-bit weights: y[r, n] = sum_k (code[n, k] - zero[n, g]) * scale[n, g] * x[r, k] with
+    g = k // group, summed in fp32 and rounded once.
+
+      codes   uint8 [E, n, k / 2]          two codes 0 .. 15 per byte, the even column in the low half
+      scales  x's dtype [E, n, k / group]  group 32, 64 or 128
+      zeros   uint8 [E, n, k / group]      zero points 0 .. 15; None: 8 everywhere
+
+    With a plan, its rows meet their expert's weights: x is [plan.capacity, k], or [T, k] with `by_token`; rows of `out`
+    [plan.capacity, n] without a pair stay as they were (in a new matrix: undefined).  Without one, codes, scales and zeros
+    are those of a single matrix (no E), and x and out have as many rows as x.
+    gated: the weights hold n / 2 linear rows, then n / 2 gated ones, and out [.., n / 2] is silu(gated) * linear.
+    x is bfloat16 or float16; n a multiple of 16, k of the group and at most 8192.  The weights are read once per eight
+    rows of an expert: for decode batches."""
+    device = _on_gpu("x", x)
+    kind = _row_type("x", x)
+    if kind == _lib.FP32:
+        raise TypeError("x must be bfloat16 or float16, got torch.float32")
+    if _wants_grad(x) or (isinstance(scales, torch.Tensor) and _wants_grad(scales)):
+        raise ValueError("matvec_w4 has no gradient: call it under torch.no_grad()")
+    if plan is not None and _check_plan(plan) != device:
+        raise ValueError(f"plan must live on {device}, got {plan.device}")
+    if by_token and plan is None:
+        raise ValueError("by_token needs a plan")
+    K = x.shape[1]
+    E = 1 if plan is None else plan.num_experts
+    if not isinstance(codes, torch.Tensor) or not isinstance(scales, torch.Tensor):
+        raise TypeError("codes and scales must be torch.Tensors")
+    lead = () if plan is None else (E,)
+    if codes.dim() != len(lead) + 2 or scales.dim() != len(lead) + 2:
+        raise ValueError(f"codes and scales must have {len(lead) + 2} dimensions{' (one matrix, no plan)' if plan is None else ''}")
+    N, G = codes.shape[-2], scales.shape[-1]
+    if G < 1 or K % G or K % 2:
+        raise ValueError(f"scales of {G} groups do not divide {K} columns")
+    cp = _packed("codes", codes, torch.uint8, (*lead, N, K // 2), device)
+    sp = _packed("scales", scales, x.dtype, (*lead, N, G), device)
+    zp = None if zeros is None else _packed("zeros", zeros, torch.uint8, (*lead, N, G), device)
+    rows = x.shape[0] if plan is None else plan.capacity
+    xp, xs = _matrix("x", x, plan.num_tokens if by_token else rows, K, x.dtype, device)
+    columns = N // 2 if gated else N
+    if out is None:
+        out = torch.empty((rows, columns), dtype=x.dtype, device=device)
+    op, os = _matrix("out", out, rows, columns, x.dtype, device)
+    _call(_lib.load().moe_fp8_b200_matvec_w4, device, xp, xs, int(by_token), C.byref(_lib.W4(cp, sp, zp, E, N, K, K // G)),
+          int(gated), op, os, kind, None if plan is None else plan._c, rows)
+    return out
+
+
 def _plain_rows(grad):
     # autograd may hand in a broadcast gradient (of a sum, say)
     return grad if grad.stride(1) == 1 else grad.contiguous()

@@ -488,6 +488,32 @@ MOE_FP8_B200_API int moe_fp8_b200_combine_rows_backward(const void* grad_out, in
                                                         const moe_fp8_b200_plan* plan, int zero_unused, void* stream,
                                                         char* err, size_t err_len);
 
+/* ---- products with 4-bit weights ------------------------------------------------------------
+ * The experts' products of a small batch with weights of half a byte (the reference's weights are e4m3 only):
+ *   y[r, n] = sum over k of (code[e, n, k] - zero[e, n, k / group]) * scale[e, n, k / group] * x[r, k]
+ * summed in fp32 and rounded once.  Codes are 0 .. 15, two per byte, the even column in the low half; without zero
+ * points the zero is 8.  `scales` and x have the same type, bf16 or fp16.
+ *   codes   [E, n, k / 2]           16-byte aligned, as are the others
+ *   scales  [E, n, k / group]
+ *   zeros   uint8 [E, n, k / group] (values 0 .. 15), or NULL
+ *   n       a multiple of 16, at most 2^20;  k a multiple of group, at most 8192;  group 32, 64 or 128 */
+typedef struct moe_fp8_b200_w4 {
+    const void* codes;
+    const void* scales;
+    const uint8_t* zeros;
+    int32_t num_experts, n, k, group;
+} moe_fp8_b200_w4;
+
+/* With a plan, row r of expert e's rows is multiplied with expert e's weights: x is [plan_rows, k], or [T, k] with
+ * by_token (row r then reads x[row_pair[r] / top_k]); out is [plan_rows, n], and rows without a pair are left as they
+ * were.  Without a plan there is one matrix (num_experts 1) and x and out have num_rows rows.
+ * gated: the weights are n / 2 linear rows followed by n / 2 gated ones, as in gemm1_weights of moe_fp8_b200_args, and out
+ * [.., n / 2] is silu(y[r, n / 2 + i]) * y[r, i] (with zero points the number of groups is then even).
+ * For decode batches: the weights are read once per eight rows of an expert.  No handle, as for the plan's functions. */
+MOE_FP8_B200_API int moe_fp8_b200_matvec_w4(const void* x, int64_t x_stride, int by_token, const moe_fp8_b200_w4* w, int gated,
+                                            void* out, int64_t out_stride, int dtype, const moe_fp8_b200_plan* plan,
+                                            int num_rows, void* stream, char* err, size_t err_len);
+
 #ifdef __cplusplus
 }
 #endif
