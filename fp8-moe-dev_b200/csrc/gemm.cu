@@ -581,6 +581,19 @@ static EncodeTiledFn get_encode_fn() {
     return fn;
 }
 
+// A tensor of `rank` dimensions of bytes or 16-bit values, the innermost contiguous; strides in bytes.
+int encode_tensor_map(void* out_map, const void* base, bool bytes, int rank, const uint64_t* dims, const uint64_t* strides,
+                      const uint32_t* box, bool swizzled)
+{
+    EncodeTiledFn fn = get_encode_fn();
+    if (!fn) return -1;
+    const cuuint32_t es[5] = {1, 1, 1, 1, 1};
+    return (int)fn(static_cast<CUtensorMap*>(out_map), bytes ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_UINT16, rank,
+                   const_cast<void*>(base), reinterpret_cast<const cuuint64_t*>(dims), reinterpret_cast<const cuuint64_t*>(strides), box,
+                   es, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzled ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE,
+                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+}
+
 // rows x K bytes (K contiguous), optionally batched over experts; box = 128 B x box_rows.
 int encode_kmajor_u8_map(void* out_map, const void* base, uint64_t k_bytes, uint64_t rows, uint64_t batch,
                          uint32_t box_rows)
