@@ -5,15 +5,29 @@
 //
 // What bounds it is the stream of the codes out of HBM: a weight is half a byte and meets at most eight rows per read.
 // The codes are read in the operator's own layout, two per byte, row by row.  One persistent CTA per SM takes a contiguous
-// range of 16-row weight tiles and keeps the next ones on their way into a ring of shared-memory stages (one TMA box per
-// tile, requested as soon as all warps have read the stage that it replaces); sixteen warps split a tile's K range and
-// multiply with mma.sync (m16n8k16: the weights are the 16-row operand, up to eight rows of x the other one).  tcgen05 has nothing to give here: its M of 128
-// would need a dequantised copy of the weights in shared memory or TMEM, and the tensor pipe is far from busy.
+// range of 16-row weight tiles.  One warp keeps the next ones on their way into a ring of shared-memory stages (one TMA box
+// per tile), sixteen warps split a tile's K range and multiply with mma.sync (the weights are the 16-row operand, the rows
+// of x the 8-column one), and three warps add up the sixteen's partial sums and store the results, so that the sixteen go
+// on with the next stage.
+// tcgen05 has nothing to give here: its M of 128 would need a converted copy of the weights in shared memory or TMEM, and
+// the tensor pipe is far from busy.
 //
-// The order of K inside a tile is free as long as both operands agree.  A thread's 32-bit word of codes holds the
-// columns 8t .. 8t+7 of a 32-column block (t = lane % 4), and the pairs (0,4) (1,5) (2,6) (3,7) fall out of it with a shift
-// and a mask each; x is held in registers in that order, loaded once per run of tiles of one expert.
-// code - zero is exact in bf16 and fp16; the products are summed in fp32, scaled per 32 columns in fp32, and rounded once.
+// What the SM has to do per byte of codes decides whether the stream runs at full rate (at 6.4 TB/s an SM gets 46 codes a
+// clock).  Two forms of the product:
+//
+// * Up to four rows of x, by integers (m16n8k32, s8).  A code becomes a signed byte with a shift and a mask per four:
+//   (code - 8) * 16 sits in the upper half of a byte already, once its top bit is flipped; with zero points the code stays
+//   in the lower half and a second product takes the zero point off.  x is split, per row and warp, into four signed
+//   bytes of a 31-bit fixed-point number below the power of two above its largest value (exact for all values down to
+//   2^-23 of that, and off by 2^-31 of it below): four columns of the product per row, so two rows per instruction.
+//   The sums of a scale's products are exact integers, and become floats by starting from 1.5 * 2^23's bit pattern.
+// * Five to eight rows, or a row with an infinity or NaN, in the type itself (m16n8k16): 0x4300 | code is 128 + code in
+//   bf16 (0x6400 | code is 1024 + code in fp16), exactly, and so is the difference to 128 + zero.  11 (9) operations
+//   per eight codes instead of 3.
+//
+// Either way the products are summed exactly or in fp32, scaled in fp32 per 32 or 64 columns, and rounded once.
+// The order of K inside a block of 32 columns is free as long as both operands agree: a thread's 32-bit word of codes
+// holds the columns 8t .. 8t+7 (t = lane % 4), and x is held in registers in the order they fall out of it.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -28,14 +42,19 @@ int encode_tensor_map(void* out_map, const void* base, bool bytes, int rank, con
 
 namespace {
 
-constexpr int kWarps = 16;
-constexpr int kThreads = kWarps * 32;
-constexpr int kLoadWarp = kWarps - 1;         // also requests the stages
+constexpr int kWarps = 16;                    // that multiply
+constexpr int kLoadWarp = kWarps;             // requests the stages
+constexpr int kSumWarps = 3;                  // add up the partial sums
+constexpr int kThreads = (kWarps + 1 + kSumWarps) * 32;
+// Registers: 640 threads x 96 at launch = 512 x 112 + 128 x 32.
+constexpr int kLaunchRegisters = 96, kMultiplyRegisters = 112, kOtherRegisters = 32;
+static_assert(kThreads * kLaunchRegisters == kWarps * 32 * kMultiplyRegisters + (1 + kSumWarps) * 32 * kOtherRegisters, "registers");
 constexpr int kTileRows = 16;                 // weight rows of a tile
 constexpr int kRowsOfX = 8;                   // rows of x that share a read of the weights
 constexpr int kMaxBlocks = 16;                // 32-column blocks of a warp
+constexpr int kFewRows = 4;                   // rows of x up to which the product goes by integers
 constexpr int kMaxK = 8192;
-constexpr int kMaxStages = 8;
+constexpr int kMaxStages = 4;
 constexpr uint32_t kSwizzleAtom = 1024;        // what the swizzle repeats after
 constexpr int kMaxExperts = MOE_FP8_B200_PLAN_MAX_EXPERTS;
 constexpr int kChunkTiles = 8;                // see Run
@@ -54,8 +73,8 @@ struct MatvecArgs {
     const int *expert_offset, *expert_count, *row_pair;   // null: one matrix, `rows` rows
     int rows;                  // rows of out
     int split, stages;         // warps that share a tile; ring
-    // A stage: the codes of its tiles, then their scales, then their zero points.  A tile's codes are `chunks` pieces of 128
-    // bytes (256 columns) of its sixteen rows, in the 128-byte swizzle (16-byte unit index XOR row mod 8).
+    // A stage: the codes of 16 / split tiles, then their scales, then their zero points.  A tile's codes are `chunks` pieces of
+    // 128 bytes (256 columns) of its sixteen rows, in the 128-byte swizzle (16-byte unit index XOR row mod 8).
     int chunks, whole;             // whole: a row is a multiple of 128 bytes, one box takes a tile
     int scale_bytes, zero_bytes;   // pitch of a row's scales and zero points
     int scale_box, zero_box;       // they come as boxes, else (rows of no multiple of 16 bytes) as they lie
@@ -72,17 +91,24 @@ struct Run {
     int expert, x_tile, tile, count;
 };
 
+// What a stage holds: `tiles` tiles from `tile` on, for `rows` rows of x and out from `row` on.  No tiles: the end.
+struct StageInfo {
+    int row, rows, tile, tiles;
+};
+// The load warp is at most kMaxStages ahead of the multiplying warps, and those two ahead of the adding ones.
+constexpr int kStageInfos = 8;
+
 struct Shared {
     int abort;
-    int warp_sum[32];
-    int first[kMaxExperts + 1];   // tiles of x rows in front of expert e
-    alignas(8) uint64_t full_bar[kMaxStages];
-    long long load_unit;          // what the load warp requests next: tiles load_done .. of the run, then this unit on
-    Run load_run;
-    int load_done;
+    int warp_sum[kThreads / 32];
+    int first[kMaxExperts + 1];                // tiles of x rows in front of expert e
+    alignas(8) uint64_t full_bar[kMaxStages];  // a stage's bytes are there
+    alignas(8) uint64_t empty_bar[kMaxStages]; // all multiplying warps have read it
+    alignas(8) uint64_t done_bar[2];           // their partial sums are there, in the buffer of the stage's parity
+    alignas(8) uint64_t free_bar[2];           // and have been added up
+    alignas(16) StageInfo info[kStageInfos];
     alignas(16) float part[2][kWarps][128];
 };
-
 
 // Work is laid out expert by expert.  An expert with more than eight rows meets its weights once per eight of them, in
 // chunks of kChunkTiles tiles, so that the second read of a chunk finds it in L2 (148 CTAs x 8 tiles x 57 KB = 68 MB).
@@ -121,6 +147,10 @@ __device__ __forceinline__ void box_load_4d(uint32_t dst, const CUtensorMap* map
                  ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(row), "r"(half), "r"(expert)
                  : "memory");
 }
+// 2^e, -149 <= e <= 127
+__device__ __forceinline__ float exp2_of(int e) {
+    return e >= -126 ? __int_as_float((e + 127) << 23) : __int_as_float(1 << (e + 149));
+}
 // (a & mask) | b in one instruction
 __device__ __forceinline__ uint32_t and_or(uint32_t a, uint32_t mask, uint32_t b) {
     uint32_t d;
@@ -152,7 +182,10 @@ template <> struct Half2<__nv_bfloat16> {
             asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(q[i]) : "r"(v), "r"(off));
         }
     }
-    static __device__ __forceinline__ float scale(uint16_t bits) { return __uint_as_float((uint32_t)bits << 16); }
+    static constexpr int kMantissa = 7, kBias = 127;
+    static constexpr uint32_t kInf = 0x7f80u;
+    static __device__ __forceinline__ float value(uint16_t bits) { return __uint_as_float((uint32_t)bits << 16); }
+    static __device__ __forceinline__ float scale(uint16_t bits) { return value(bits); }
     static __device__ __forceinline__ __nv_bfloat16 round(float v) { return __float2bfloat16_rn(v); }
 };
 template <> struct Half2<__half> {
@@ -177,12 +210,27 @@ template <> struct Half2<__half> {
             asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(q[2 * i + 1]) : "r"(hi), "r"(0x2c002c00u), "r"(neg));
         }
     }
-    static __device__ __forceinline__ float scale(uint16_t bits) { return __half2float(__ushort_as_half(bits)); }
+    static constexpr int kMantissa = 10, kBias = 15;
+    static constexpr uint32_t kInf = 0x7c00u;
+    static __device__ __forceinline__ float value(uint16_t bits) { return __half2float(__ushort_as_half(bits)); }
+    static __device__ __forceinline__ float scale(uint16_t bits) { return value(bits); }
     static __device__ __forceinline__ __half round(float v) { return __float2half_rn(v); }
 };
 
+__device__ __forceinline__ void mma_s8(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// (a ^ b) & mask in one instruction
+__device__ __forceinline__ uint32_t xor_and(uint32_t a, uint32_t b, uint32_t mask) {
+    uint32_t d;
+    asm("lop3.b32 %0, %1, %2, %3, 0x28;" : "=r"(d) : "r"(a), "r"(b), "r"(mask));
+    return d;
+}
+
 // A thread's part of a tile in shared memory (bytes into the ring).  A warp takes every split-th pair of 32-column blocks,
-// so that its pairs lie at one distance: split / 4 chunks.
+// so that its pairs lie at one distance, split / 4 chunks.
 struct TileView {
     const uint8_t* ring;
     int even, odd;     // its word of the first pair's two blocks in weight row g; row g + 8 lies 1024 bytes further
@@ -192,61 +240,238 @@ struct TileView {
     int last_scale, last_zero;   // of the row: a pair's second block may lie behind the last column, where x is zero
 };
 
-// COUNT pairs of blocks from pair FIRST on, in one stretch without a branch, so that their loads, conversions and matrix
-// instructions overlap.  The products of a pair are summed in fp32 by the matrix instructions, one scale at a time
-// (FINE: two scales in a pair).
-template <typename H, bool FINE, bool ZEROS, int FIRST, int COUNT, int BLOCKS>
-__device__ __forceinline__ void multiply_pairs(float (&acc)[4], const uint32_t (&xr)[BLOCKS][4], const TileView& v)
-{
-    constexpr int kScales = FINE ? 2 : 1, kBlocks = 2 / kScales;   // scales of a pair, blocks of a scale
-    uint32_t w0[2 * COUNT], w1[2 * COUNT];
+// The words of COUNT pairs of blocks from `pair` on, and the scales and zero points of one.
+template <int COUNT>
+struct Words {
+    uint32_t row0[2 * COUNT], row1[2 * COUNT];
+    __device__ __forceinline__ Words(const TileView& v, int pair) {
 #pragma unroll
-    for (int p = 0; p < COUNT; ++p) {
-        const int at = (FIRST + p) * v.pair_step;
-        w0[2 * p] = *reinterpret_cast<const uint32_t*>(v.ring + v.even + at);
-        w1[2 * p] = *reinterpret_cast<const uint32_t*>(v.ring + v.even + at + 1024);
-        w0[2 * p + 1] = *reinterpret_cast<const uint32_t*>(v.ring + v.odd + at);
-        w1[2 * p + 1] = *reinterpret_cast<const uint32_t*>(v.ring + v.odd + at + 1024);
-    }
-#pragma unroll
-    for (int p = 0; p < COUNT; ++p)
-#pragma unroll
-        for (int i = 0; i < kScales; ++i) {
-            int sa = v.scales + (FIRST + p) * v.scale_step, za = v.zeros + (FIRST + p) * v.zero_step;
-            if (i) {
-                sa = min(sa + 2, v.last_scale);
-                za = min(za + 1, v.last_zero);
-            }
-            const float s0 = H::scale(*reinterpret_cast<const uint16_t*>(v.ring + sa));
-            const float s1 = H::scale(*reinterpret_cast<const uint16_t*>(v.ring + sa + v.scale_rows));
-            const uint32_t off0 = H::offset(ZEROS ? v.ring[za] : 8u), off1 = H::offset(ZEROS ? v.ring[za + v.zero_rows] : 8u);
-            float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-            for (int j = 2 * p + i * kBlocks; j < 2 * p + (i + 1) * kBlocks; ++j) {
-                uint32_t q0[4], q1[4];
-                H::decode(w0[j], off0, q0);
-                H::decode(w1[j], off1, q1);
-                H::mma(c, c, q0[0], q1[0], q0[1], q1[1], xr[2 * FIRST + j][0], xr[2 * FIRST + j][1]);
-                H::mma(c, c, q0[2], q1[2], q0[3], q1[3], xr[2 * FIRST + j][2], xr[2 * FIRST + j][3]);
-            }
-            acc[0] = fmaf(s0, c[0], acc[0]);
-            acc[1] = fmaf(s0, c[1], acc[1]);
-            acc[2] = fmaf(s1, c[2], acc[2]);
-            acc[3] = fmaf(s1, c[3], acc[3]);
+        for (int p = 0; p < COUNT; ++p) {
+            const int at = (pair + p) * v.pair_step;
+            row0[2 * p] = *reinterpret_cast<const uint32_t*>(v.ring + v.even + at);
+            row1[2 * p] = *reinterpret_cast<const uint32_t*>(v.ring + v.even + at + 1024);
+            row0[2 * p + 1] = *reinterpret_cast<const uint32_t*>(v.ring + v.odd + at);
+            row1[2 * p + 1] = *reinterpret_cast<const uint32_t*>(v.ring + v.odd + at + 1024);
         }
+    }
+};
+// `second`: the pair's second scale
+template <typename H, bool ZEROS>
+struct Scales {
+    float s0, s1;
+    uint32_t z0, z1;
+    __device__ __forceinline__ Scales(const TileView& v, int pair, bool second) {
+        int sa = v.scales + pair * v.scale_step, za = v.zeros + pair * v.zero_step;
+        if (second) {
+            sa = min(sa + 2, v.last_scale);
+            za = min(za + 1, v.last_zero);
+        }
+        s0 = H::scale(*reinterpret_cast<const uint16_t*>(v.ring + sa));
+        s1 = H::scale(*reinterpret_cast<const uint16_t*>(v.ring + sa + v.scale_rows));
+        z0 = ZEROS ? v.ring[za] : 8u;
+        z1 = ZEROS ? v.ring[za + v.zero_rows] : 8u;
+    }
+};
+
+// COUNT pairs of blocks from pair FIRST on, in one stretch without a branch, so that their loads, conversions and matrix
+// instructions overlap.  The products of a pair are summed by the matrix
+// instructions, one scale at a time (FINE: two scales in a pair).  Here in the type itself, for eight rows of x.
+template <typename H, bool FINE, bool ZEROS>
+struct ByType {
+    template <int FIRST, int COUNT>
+    static __device__ __forceinline__ void multiply(float (&acc)[8], const uint32_t (&xr)[kMaxBlocks][4], const TileView& v) {
+        constexpr int kScales = FINE ? 2 : 1, kBlocks = 2 / kScales;   // scales of a pair, blocks of a scale
+        const Words<COUNT> w(v, FIRST);
+#pragma unroll
+        for (int p = 0; p < COUNT; ++p)
+#pragma unroll
+            for (int i = 0; i < kScales; ++i) {
+                const Scales<H, ZEROS> s(v, FIRST + p, i != 0);
+                const uint32_t off0 = H::offset(s.z0), off1 = H::offset(s.z1);
+                float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int j = 2 * p + i * kBlocks; j < 2 * p + (i + 1) * kBlocks; ++j) {
+                    const uint32_t(&x)[4] = xr[2 * FIRST + j];
+                    uint32_t q0[4], q1[4];
+                    H::decode(w.row0[j], off0, q0);
+                    H::decode(w.row1[j], off1, q1);
+                    H::mma(c, c, q0[0], q1[0], q0[1], q1[1], x[0], x[1]);
+                    H::mma(c, c, q0[2], q1[2], q0[3], q1[3], x[2], x[3]);
+                }
+                acc[0] = fmaf(s.s0, c[0], acc[0]);
+                acc[1] = fmaf(s.s0, c[1], acc[1]);
+                acc[2] = fmaf(s.s1, c[2], acc[2]);
+                acc[3] = fmaf(s.s1, c[3], acc[3]);
+            }
+    }
+};
+
+// By integers, for 2 * MMAS rows of x: column 4 r + d of a product is byte d of row r.  At most 64 products of 2^7 by 2^7 meet in
+// a sum, so it stays below 2^22 and kOne + sum is a float's bit pattern whose value is 1.5 * 2^23 + sum.
+template <typename H, bool FINE, bool ZEROS, int MMAS>
+struct ByInteger {
+    static constexpr int kOne = 0x4b400000;
+    template <int FIRST, int COUNT>
+    static __device__ __forceinline__ void multiply(float (&acc)[8], const uint32_t (&xr)[kMaxBlocks][4], const TileView& v) {
+        constexpr int kScales = FINE ? 2 : 1, kBlocks = 2 / kScales;
+        const Words<COUNT> w(v, FIRST);
+#pragma unroll
+        for (int p = 0; p < COUNT; ++p)
+#pragma unroll
+            for (int i = 0; i < kScales; ++i) {
+                const Scales<H, ZEROS> s(v, FIRST + p, i != 0);
+                const uint32_t neg0 = (0u - s.z0 & 0xffu) * 0x01010101u, neg1 = (0u - s.z1 & 0xffu) * 0x01010101u;   // bytes -zero
+                int c[MMAS][4];
+#pragma unroll
+                for (int m = 0; m < MMAS; ++m) c[m][0] = c[m][1] = c[m][2] = c[m][3] = kOne;
+#pragma unroll
+                for (int j = 2 * p + i * kBlocks; j < 2 * p + (i + 1) * kBlocks; ++j) {
+                    const uint32_t(&x)[4] = xr[2 * FIRST + j];
+                    uint32_t even0, odd0, even1, odd1;
+                    if (ZEROS) {
+                        even0 = w.row0[j] & 0x0f0f0f0fu, odd0 = (w.row0[j] >> 4) & 0x0f0f0f0fu;
+                        even1 = w.row1[j] & 0x0f0f0f0fu, odd1 = (w.row1[j] >> 4) & 0x0f0f0f0fu;
+                    } else {
+                        even0 = xor_and(w.row0[j] << 4, 0x80808080u, 0xf0f0f0f0u), odd0 = xor_and(w.row0[j], 0x80808080u, 0xf0f0f0f0u);
+                        even1 = xor_and(w.row1[j] << 4, 0x80808080u, 0xf0f0f0f0u), odd1 = xor_and(w.row1[j], 0x80808080u, 0xf0f0f0f0u);
+                    }
+#pragma unroll
+                    for (int m = 0; m < MMAS; ++m) {
+                        mma_s8(c[m], even0, even1, odd0, odd1, x[2 * m], x[2 * m + 1]);
+                        if (ZEROS) mma_s8(c[m], neg0, neg1, neg0, neg1, x[2 * m], x[2 * m + 1]);
+                    }
+                }
+#pragma unroll
+                for (int m = 0; m < MMAS; ++m)
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        acc[4 * m + k] = fmaf(k < 2 ? s.s0 : s.s1, __int_as_float(c[m][k]) - __int_as_float(kOne), acc[4 * m + k]);
+            }
+    }
+};
+
+// All of a warp's pairs, two at a time.
+template <typename P, int FIRST = 0>
+__device__ __forceinline__ void multiply_pairs(float (&acc)[8], const uint32_t (&xr)[kMaxBlocks][4], const TileView& v, int pairs)
+{
+    if constexpr (2 * FIRST < kMaxBlocks) {
+        if (pairs >= FIRST + 2) {
+            P::template multiply<FIRST, 2>(acc, xr, v);
+            multiply_pairs<P, FIRST + 2>(acc, xr, v, pairs);
+        } else if (pairs > FIRST) {
+            P::template multiply<FIRST, 1>(acc, xr, v);
+        }
+    }
 }
 
-template <typename H, bool FINE, bool ZEROS, int FIRST, int BLOCKS>
-__device__ __forceinline__ void multiply_from(float (&acc)[4], const uint32_t (&xr)[BLOCKS][4], const TileView& v, int pairs)
+// Row `i` of a run's x, from its member-th pair of blocks on.
+__device__ __forceinline__ const uint8_t* x_row(const MatvecArgs& a, int row, int rows, int i, int member) {
+    int src = row + min(i, rows - 1);
+    if (a.by_token) src = a.row_pair[src] / a.top_k;
+    src = min(max(src, 0), a.x_rows - 1);
+    return a.x + src * a.x_stride + member * 128;
+}
+
+// x for the products in its own type: thread (g, t) holds row g's columns 8t .. 8t+7 of each of its warp's blocks, as the pairs
+// (0, 4) (1, 5) (2, 6) (3, 7); zeros behind the last column.  A row of bf16 values near the end of fp32's range is held 2^16
+// times smaller, so that products with codes do not leave it; `unit` says so for rows 2t and 2t + 1.
+template <typename T>
+__device__ __forceinline__ void load_values(uint32_t (&xr)[kMaxBlocks][4], float (&unit)[2], const MatvecArgs& a, int row, int rows,
+                                            int member, int lane)
 {
-    if constexpr (2 * FIRST < BLOCKS) {
-        if (pairs >= FIRST + 2) {
-            multiply_pairs<H, FINE, ZEROS, FIRST, 2>(acc, xr, v);
-            multiply_from<H, FINE, ZEROS, FIRST + 2>(acc, xr, v, pairs);
-        } else if (pairs > FIRST) {
-            multiply_pairs<H, FINE, ZEROS, FIRST, 1>(acc, xr, v);
+    const int g = lane / 4, t = lane % 4;
+    const uint8_t* xp = x_row(a, row, rows, g, member) + 16 * t;
+#pragma unroll
+    for (int j = 0; j < kMaxBlocks; ++j) {
+        uint32_t v[4] = {0, 0, 0, 0};
+        const int block = 2 * (member + j / 2 * a.split) + j % 2, at = (block - 2 * member) * 64;
+        if (block * 32 < a.K) {
+            if (a.x_wide) {
+                const uint4 q = *reinterpret_cast<const uint4*>(xp + at);
+                v[0] = q.x; v[1] = q.y; v[2] = q.z; v[3] = q.w;
+            } else {
+                const uint16_t* h = reinterpret_cast<const uint16_t*>(xp + at);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) v[i] = (uint32_t)h[2 * i] | ((uint32_t)h[2 * i + 1] << 16);
+            }
+        }
+        xr[j][0] = __byte_perm(v[0], v[2], 0x5410);
+        xr[j][1] = __byte_perm(v[0], v[2], 0x7632);
+        xr[j][2] = __byte_perm(v[1], v[3], 0x5410);
+        xr[j][3] = __byte_perm(v[1], v[3], 0x7632);
+    }
+    unit[0] = unit[1] = 1.0f;
+    if constexpr (Half2<T>::kMantissa == 7) {
+        uint32_t most = 0;
+#pragma unroll
+        for (int j = 0; j < kMaxBlocks; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) most = max(most, max(xr[j][i] & 0x7fffu, xr[j][i] >> 16 & 0x7fffu));
+        most = max(most, __shfl_xor_sync(~0u, most, 1));
+        most = max(most, __shfl_xor_sync(~0u, most, 2));
+        const bool large = most >= (112u + 127u) << 7;
+        if (__any_sync(~0u, large)) {
+            const uint32_t by = large ? 0x37803780u : 0x3f803f80u;   // 2^-16 or 1, twice
+#pragma unroll
+            for (int j = 0; j < kMaxBlocks; ++j)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) asm("mul.rn.bf16x2 %0, %0, %1;" : "+r"(xr[j][i]) : "r"(by));
+            const unsigned rows_large = __ballot_sync(~0u, large);
+            if (rows_large >> (8 * t) & 1) unit[0] = 65536.0f;
+            if (rows_large >> (8 * t + 4) & 1) unit[1] = 65536.0f;
         }
     }
+}
+
+// x for the products by integers: thread (g, t) holds byte g % 4 of rows g / 4 and 2 + g / 4, of the columns 8t, 8t+2, 8t+4,
+// 8t+6 in one word and of the odd ones in the next.  A value is 31 bits below 2^e, the power of two above the largest of
+// its row's values in this warp, split into signed bytes.  Each thread converts two columns of a block; four threads'
+// words are then transposed byte by byte.  Returns the form that x is in (1 up to two rows, 2 up to four), or 0 if a value
+// is not finite.
+template <typename T>
+__device__ __forceinline__ int load_digits(uint32_t (&xr)[kMaxBlocks][4], float (&unit)[2], const MatvecArgs& a, int row, int rows,
+                                           int member, int lane)
+{
+    const int t = lane % 4, q = lane / 4 % 4, forms = rows <= 2 ? 1 : 2;
+    const uint32_t swap2 = q < 2 ? 0x5410u : 0x3276u, swap1 = q & 1 ? 0x3715u : 0x6240u;
+#pragma unroll
+    for (int m = 0; m < 2; ++m) {
+        if (m >= forms) break;
+        const uint8_t* xp = x_row(a, row, rows, 2 * m + lane / 16, member) + 16 * t + 4 * q;
+        uint32_t raw[kMaxBlocks], most = 0;
+#pragma unroll
+        for (int j = 0; j < kMaxBlocks; ++j) {
+            const int block = 2 * (member + j / 2 * a.split) + j % 2, at = (block - 2 * member) * 64;
+            raw[j] = 0;
+            if (block * 32 < a.K) {
+                if (a.x_wide) {
+                    raw[j] = *reinterpret_cast<const uint32_t*>(xp + at);
+                } else {
+                    const uint16_t* h = reinterpret_cast<const uint16_t*>(xp + at);
+                    raw[j] = (uint32_t)h[0] | ((uint32_t)h[1] << 16);
+                }
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < kMaxBlocks; ++j) most = max(most, max(raw[j] & 0x7fffu, raw[j] >> 16 & 0x7fffu));
+#pragma unroll
+        for (int d = 1; d < 16; d <<= 1) most = max(most, __shfl_xor_sync(~0u, most, d));
+        if (__any_sync(~0u, most >= Half2<T>::kInf)) return 0;
+        const int e = (int)(most >> Half2<T>::kMantissa) - Half2<T>::kBias + 1;   // all below 2^e
+        const float scale = exp2_of(-e);
+        unit[m] = exp2_of(__shfl_sync(~0u, e, (t >> 1) * 16) - 1);
+#pragma unroll
+        for (int j = 0; j < kMaxBlocks; ++j)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const float x = Half2<T>::value((uint16_t)(raw[j] >> (16 * i)));
+                uint32_t v = ((uint32_t)__float2int_rn(x * scale * 0x1p30f) + 0x80808080u) ^ 0x80808080u;   // bytes -128 .. 127
+                v = __byte_perm(v, __shfl_xor_sync(~0u, v, 8), swap2);
+                v = __byte_perm(v, __shfl_xor_sync(~0u, v, 4), swap1);
+                xr[j][2 * m + i] = v;
+            }
+    }
+    return forms;
 }
 
 template <typename T, bool GATED, bool FINE, bool ZEROS>
@@ -261,7 +486,14 @@ __global__ void __launch_bounds__(kThreads, 1) matvec4_kernel(const MatvecArgs a
     pdl_launch_dependents();
     if (threadIdx.x == 0) {
         sh.abort = 0;
-        for (int i = 0; i < a.stages; ++i) mbar_init(smem_u32(&sh.full_bar[i]), 1);
+        for (int i = 0; i < a.stages; ++i) {
+            mbar_init(smem_u32(&sh.full_bar[i]), 1);
+            mbar_init(smem_u32(&sh.empty_bar[i]), kWarps);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(smem_u32(&sh.done_bar[i]), kWarps);
+            mbar_init(smem_u32(&sh.free_bar[i]), kSumWarps);
+        }
         fence_mbar_init();
     }
     __syncthreads();
@@ -286,7 +518,7 @@ __global__ void __launch_bounds__(kThreads, 1) matvec4_kernel(const MatvecArgs a
             if (lane == 31) sh.warp_sum[warp] = upto;
             __syncthreads();
             int total = 0;
-            for (int w = 0; w < kWarps; ++w) {
+            for (int w = 0; w < kThreads / 32; ++w) {
                 if (w < warp) upto += sh.warp_sum[w];
                 total += sh.warp_sum[w];
             }
@@ -305,65 +537,117 @@ __global__ void __launch_bounds__(kThreads, 1) matvec4_kernel(const MatvecArgs a
     const long long units = (long long)sh.first[a.E] * tiles;
     const long long begin = units * blockIdx.x / gridDim.x, end = units * (blockIdx.x + 1) / gridDim.x;
 
-    // Requests one stage: one weight row per lane, then the scales and zero points.  Only the load warp calls it.
-    auto request_stage = [&](int slot) {
-        if (sh.load_done == sh.load_run.count) {
-            const long long u = sh.load_unit;
-            if (u >= end) return;
-            const Run next = run_at(sh, a, u, end, tiles);
-            __syncwarp();
-            if (lane == 0) {
-                sh.load_run = next;
-                sh.load_unit = u + next.count;
-                sh.load_done = 0;
-            }
-            __syncwarp();
+    // The rows of x and out that a run's tiles meet.
+    auto rows_of = [&](const Run& r) {
+        int first = 0, count = a.rows;
+        if (a.expert_count) {
+            first = a.expert_offset[r.expert];
+            count = min(a.expert_count[r.expert], a.rows - first);
         }
-        const Run r = sh.load_run;
-        const int t0 = sh.load_done, n = min(per_stage, r.count - t0);
-        const uint32_t bar = smem_u32(&sh.full_bar[slot]), dst = ring0 + slot * a.stage_bytes;
-        __syncwarp();
-        if (lane == 0) {
-            sh.load_done = t0 + n;
-            const int codes = a.chunks * 128, scales = a.scale_box ? a.scale_bytes : groups * 2, zeros = a.zero_box ? a.zero_bytes : groups;
-            mbar_expect_tx(bar, (uint32_t)(n * kTileRows) * (uint32_t)(codes + scales + (ZEROS ? zeros : 0)));
-        }
-        __syncwarp();
-        const int rows = GATED ? kTileRows / 2 : kTileRows;
-        // a tile's scales where they are no box: as they lie, in two halves if gated
-        auto copy_side = [&](const uint8_t* src, int bytes, int tile, uint32_t to) {
-            for (int half = 0; half < (GATED ? 2 : 1); ++half)
-                bulk_load(to + half * rows * bytes, src + ((long long)r.expert * a.N + half * (a.N / 2) + tile * rows) * bytes,
-                          rows * bytes, bar);
-        };
-        const int boxes = a.whole ? 1 : a.chunks;
-        for (int i = lane; i < n * boxes; i += 32) {
-            const int m = i / boxes, c = i - m * boxes;
-            box_load_5d(dst + (m * a.chunks + c) * 2048, &maps.codes, bar, a.whole ? 0 : c * 128, (r.tile + t0 + m) * rows, 0, 0, r.expert);
-        }
-        for (int m = lane; m < n; m += 32) {
-            const int tile = r.tile + t0 + m;
-            const uint32_t to = dst + a.scale_at + m * kTileRows * a.scale_bytes;
-            if (a.scale_box) box_load_4d(to, &maps.scales, bar, 0, tile * rows, 0, r.expert);
-            else copy_side(a.scales, groups * 2, tile, to);
-            if (ZEROS) {
-                const uint32_t zero_to = dst + a.zero_at + m * kTileRows * a.zero_bytes;
-                if (a.zero_box) box_load_4d(zero_to, &maps.zeros, bar, 0, tile * rows, 0, r.expert);
-                else copy_side(a.zeros, groups, tile, zero_to);
-            }
-        }
+        return make_int2(first + r.x_tile * kRowsOfX, min(kRowsOfX, count - r.x_tile * kRowsOfX));
     };
-    if (warp == kLoadWarp) {
-        if (lane == 0) {
-            prefetch_tmap(&maps.codes);
-            sh.load_unit = begin;
-            sh.load_done = sh.load_run.count = 0;
+    bool ok = true;
+
+    if (warp >= kWarps) {
+        setmaxnreg_dec<kOtherRegisters>();
+        if (warp == kLoadWarp) {
+            // ---- the stages, one after the other, and the end
+            if (lane == 0) prefetch_tmap(&maps.codes);
+            const int rows = GATED ? kTileRows / 2 : kTileRows;
+            int it = 0, slot = 0, lap = 0;
+            auto advance = [&] {
+                ++it;
+                if (++slot == a.stages) {
+                    slot = 0;
+                    lap ^= 1;
+                }
+            };
+            for (long long u = begin; u < end && ok;) {
+                const Run r = run_at(sh, a, u, end, tiles);
+                const int2 x = rows_of(r);
+                u += r.count;
+                for (int t0 = 0; t0 < r.count; t0 += per_stage, advance()) {
+                    ok = it < a.stages || mbar_wait(smem_u32(&sh.empty_bar[slot]), lap ^ 1, &sh.abort);
+                    if (!__all_sync(~0u, ok)) { ok = false; break; }
+                    const int n = min(per_stage, r.count - t0);
+                    const uint32_t bar = smem_u32(&sh.full_bar[slot]), dst = ring0 + slot * a.stage_bytes;
+                    if (lane == 0) {
+                        sh.info[it % kStageInfos] = {x.x, x.y, r.tile + t0, n};
+                        const int scales = a.scale_box ? a.scale_bytes : groups * 2, zeros = a.zero_box ? a.zero_bytes : groups;
+                        mbar_expect_tx(bar, (uint32_t)(n * kTileRows) * (uint32_t)(a.chunks * 128 + scales + (ZEROS ? zeros : 0)));
+                    }
+                    __syncwarp();
+                    const int boxes = a.whole ? 1 : a.chunks;
+                    for (int i = lane; i < n * boxes; i += 32) {
+                        const int m = i / boxes, c = i - m * boxes;
+                        box_load_5d(dst + (m * a.chunks + c) * 2048, &maps.codes, bar, c * 128, (r.tile + t0 + m) * rows, 0, 0, r.expert);
+                    }
+                    // a tile's scales where they are no box: as they lie, in two halves if gated
+                    auto copy_side = [&](const uint8_t* src, int bytes, int tile, uint32_t to) {
+                        for (int half = 0; half < (GATED ? 2 : 1); ++half)
+                            bulk_load(to + half * rows * bytes, src + ((long long)r.expert * a.N + half * (a.N / 2) + tile * rows) * bytes,
+                                      rows * bytes, bar);
+                    };
+                    for (int m = lane; m < n; m += 32) {
+                        const int tile = r.tile + t0 + m;
+                        const uint32_t to = dst + a.scale_at + m * kTileRows * a.scale_bytes;
+                        if (a.scale_box) box_load_4d(to, &maps.scales, bar, 0, tile * rows, 0, r.expert);
+                        else copy_side(a.scales, groups * 2, tile, to);
+                        if (ZEROS) {
+                            const uint32_t zero_to = dst + a.zero_at + m * kTileRows * a.zero_bytes;
+                            if (a.zero_box) box_load_4d(zero_to, &maps.zeros, bar, 0, tile * rows, 0, r.expert);
+                            else copy_side(a.zeros, groups, tile, zero_to);
+                        }
+                    }
+                }
+            }
+            if (ok) ok = it < a.stages || mbar_wait(smem_u32(&sh.empty_bar[slot]), lap ^ 1, &sh.abort);
+            if (ok && lane == 0) {
+                sh.info[it % kStageInfos].tiles = 0;
+                mbar_arrive(smem_u32(&sh.full_bar[slot]));
+            }
+            if (!ok) {
+                // A wait of a second ran out (see mbar_wait): nothing of this CTA stays on its way.
+                int waited = 0;
+                for (int i = 0; i < a.stages; ++i) {
+                    slot = slot == 0 ? a.stages - 1 : slot - 1;
+                    if (slot == a.stages - 1) lap ^= 1;
+                    if (it - 1 - i >= 0) mbar_wait(smem_u32(&sh.full_bar[slot]), lap, &waited);
+                }
+            }
+        } else {
+            // ---- results of a stage: 128 per tile, the sums of its `split` warps' partial sums.  Thread (i, lane) has weight row
+            // g + 8 (i / 2) and x row 2t + i % 2.
+            const int g = lane / 4, t = lane % 4;
+            for (int it = 0;; ++it) {
+                const int b = it & 1;
+                ok = mbar_wait(smem_u32(&sh.done_bar[b]), (it >> 1) & 1, &sh.abort);
+                if (!ok) break;
+                const StageInfo s = sh.info[it % kStageInfos];
+                if (s.tiles == 0) break;
+                const float(*part)[128] = sh.part[b];
+                for (int v = warp - kLoadWarp - 1; v < s.tiles * (GATED ? 2 : 4); v += kSumWarps) {
+                    const int m = GATED ? v / 2 : v / 4, i = GATED ? v % 2 : v % 4, x_row = 2 * t + (i & 1);
+                    float y = 0.0f, gate = 0.0f;
+                    for (int k = 0; k < a.split; ++k) {
+                        y += part[m * a.split + k][i * 32 + lane];
+                        if (GATED) gate += part[m * a.split + k][(i + 2) * 32 + lane];
+                    }
+                    if (x_row < s.rows) {
+                        if (GATED) y = gate / (1.0f + __expf(-gate)) * y;
+                        const int col = GATED ? (s.tile + m) * 8 + g : (s.tile + m) * kTileRows + g + 8 * (i / 2);
+                        reinterpret_cast<T*>(a.out + (s.row + x_row) * a.out_stride)[col] = H::round(y);
+                    }
+                }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(smem_u32(&sh.free_bar[b]));
+            }
         }
-        __syncwarp();
-        for (int i = 0; i < a.stages; ++i) request_stage(i);
+        return;
     }
 
-    // `split` warps share a tile's K range, tile m of the stage belongs to warps [m * split, (m + 1) * split)
+    // ---- `split` warps share a tile's K range, tile m of the stage belongs to warps [m * split, (m + 1) * split)
+    setmaxnreg_inc<kMultiplyRegisters>();
     const int member = warp % a.split, of_stage = warp / a.split;
     // every split-th pair of 32-column blocks; the last pair of an odd number of blocks has its second block's x zero
     const int all_pairs = (a.K + 63) / 64, pairs = (all_pairs - member + a.split - 1) / a.split;
@@ -387,80 +671,77 @@ __global__ void __launch_bounds__(kThreads, 1) matvec4_kernel(const MatvecArgs a
         view.last_zero = a.zero_at + row * a.zero_bytes + groups - 1;
     }
     uint32_t xr[kMaxBlocks][4];
-    int it = 0;
-    bool ok = true;
-    for (long long u = begin; u < end;) {
-        const Run r = run_at(sh, a, u, end, tiles);
-        u += r.count;
-        // rows of x of this run, in the order the codes come out of a word
-        const int row0 = (a.expert_count ? a.expert_offset[r.expert] : 0) + r.x_tile * kRowsOfX;
-        const int rows = min(kRowsOfX, (a.expert_count ? min(a.expert_count[r.expert], a.rows - a.expert_offset[r.expert]) : a.rows) -
-                                           r.x_tile * kRowsOfX);
-        {
-            int src = row0 + min(g, rows - 1);
-            if (a.by_token) src = a.row_pair[src] / a.top_k;
-            src = min(max(src, 0), a.x_rows - 1);
-            const uint8_t* xp = a.x + src * a.x_stride + (member * 64 + 8 * t) * 2;
+    int form = 0;                      // 0 in the type itself, 1 by integers for up to two rows, 2 for up to four
+    // by integers, half of the power of two above the largest value of rows t / 2 and 2 + t / 2 of x; else see load_values
+    float unit[2] = {0.0f, 0.0f};
+    int slot = 0, lap = 0, row = -1;
+    for (int it = 0;; ++it) {
+        ok = mbar_wait(smem_u32(&sh.full_bar[slot]), lap, &sh.abort);
+        if (!ok) break;
+        const StageInfo s = sh.info[it % kStageInfos];
+        const int b = it & 1;
+        if (s.tiles == 0) {
+            // the adding warps see the end, too; not before all have arrived for the stage two before it
+            if (it >= 2) ok = mbar_wait(smem_u32(&sh.free_bar[b]), (it >> 1) - 1 & 1, &sh.abort);
+            if (ok && lane == 0) mbar_arrive(smem_u32(&sh.done_bar[b]));
+            break;
+        }
+        if (s.row != row) {
+            row = s.row;
+            form = 0;
+            if (s.rows <= kFewRows) form = load_digits<T>(xr, unit, a, row, s.rows, member, lane);
+            if (form == 0) load_values<T>(xr, unit, a, row, s.rows, member, lane);
+        }
+        float acc[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+        if (of_stage < s.tiles) {
+            TileView v = view;
+            const int at = slot * a.stage_bytes;
+            v.even += at;
+            v.odd += at;
+            v.scales += at;
+            v.zeros += at;
+            v.last_scale += at;
+            v.last_zero += at;
+            if (form == 1) multiply_pairs<ByInteger<H, FINE, ZEROS, 1>>(acc, xr, v, pairs);
+            else if (form == 2) multiply_pairs<ByInteger<H, FINE, ZEROS, 2>>(acc, xr, v, pairs);
+            else multiply_pairs<ByType<H, FINE, ZEROS>>(acc, xr, v, pairs);
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&sh.empty_bar[slot]));
+        if (it >= 2) ok = mbar_wait(smem_u32(&sh.free_bar[b]), (it >> 1) - 1 & 1, &sh.abort);
+        if (!ok) break;
+        float* part = sh.part[b][warp];
+        if (form == 0) {
 #pragma unroll
-            for (int j = 0; j < kMaxBlocks; ++j) {
-                uint32_t v[4] = {0, 0, 0, 0};
-                const int block = 2 * (member + j / 2 * a.split) + j % 2, at = (block - 2 * member) * 64;
-                if (block * 32 < a.K) {
-                    if (a.x_wide) {
-                        const uint4 q = *reinterpret_cast<const uint4*>(xp + at);
-                        v[0] = q.x; v[1] = q.y; v[2] = q.z; v[3] = q.w;
-                    } else {
-                        const uint16_t* h = reinterpret_cast<const uint16_t*>(xp + at);
+            for (int i = 0; i < 4; ++i) part[i * 32 + lane] = acc[i] * unit[i & 1];
+        } else {
+            // this thread's columns 2t, 2t + 1 are bytes 0, 1 (t even) or 2, 3 of x row t / 2 (and 2 + t / 2)
+            const float low = (t & 1 ? 65536.0f : 1.0f) * (ZEROS ? 0x1p-29f : 0x1p-33f);
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) v[i] = (uint32_t)h[2 * i] | ((uint32_t)h[2 * i + 1] << 16);
-                    }
-                }
-                xr[j][0] = __byte_perm(v[0], v[2], 0x5410);   // (0, 4)
-                xr[j][1] = __byte_perm(v[0], v[2], 0x7632);   // (1, 5)
-                xr[j][2] = __byte_perm(v[1], v[3], 0x5410);   // (2, 6)
-                xr[j][3] = __byte_perm(v[1], v[3], 0x7632);   // (3, 7)
+            for (int m = 0; m < 2; ++m) {
+                if (m >= form) break;
+                float y0 = fmaf(256.0f, acc[4 * m + 1], acc[4 * m]) * low * unit[m];
+                float y1 = fmaf(256.0f, acc[4 * m + 3], acc[4 * m + 2]) * low * unit[m];
+                y0 += __shfl_xor_sync(~0u, y0, 1);
+                y1 += __shfl_xor_sync(~0u, y1, 1);
+                part[((t & 1) * 2 + (t >> 1)) * 32 + g * 4 + m] = t & 1 ? y1 : y0;
             }
         }
-        for (int t0 = 0; t0 < r.count; t0 += per_stage, ++it) {
-            const int slot = it % a.stages, n = min(per_stage, r.count - t0);
-            ok = mbar_wait(smem_u32(&sh.full_bar[slot]), (it / a.stages) & 1, &sh.abort) && ok;
-            float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-            if (of_stage < n && ok) {
-                TileView v = view;
-                const int stage = slot * a.stage_bytes;
-                v.even += stage;
-                v.odd += stage;
-                v.scales += stage;
-                v.zeros += stage;
-                v.last_scale += stage;
-                v.last_zero += stage;
-                multiply_from<H, FINE, ZEROS, 0>(acc, xr, v, pairs);
-            }
-            // the tile's partial sums meet (two buffers, so one barrier per stage), and the stage has been read
-            float(*part)[128] = sh.part[it & 1];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) part[warp][i * 32 + lane] = acc[i];
-            __syncthreads();
-            if (warp == kLoadWarp && ok) request_stage(slot);
-            // 128 results per tile, added up by the warps in turn: thread (i, lane) has row g + 8 (i / 2), x row 2t + i % 2
-            const int first = (it * 4) % kWarps;
-            for (int v = (warp + kWarps - first) % kWarps; v < n * 4; v += kWarps) {
-                const int m = v / 4, i = v % 4;
-                if (GATED && i >= 2) continue;
-                float y = 0.0f, gate = 0.0f;
-                for (int k = 0; k < a.split; ++k) {
-                    y += part[m * a.split + k][i * 32 + lane];
-                    if (GATED) gate += part[m * a.split + k][(i + 2) * 32 + lane];
-                }
-                const int xrow = 2 * t + (i & 1);
-                if (xrow < rows) {
-                    if (GATED) y = gate / (1.0f + __expf(-gate)) * y;
-                    if (!ok) y = __int_as_float(0x7fc00000);   // a load that never came
-                    const int tile = r.tile + t0 + m;
-                    const int col = GATED ? tile * 8 + g : tile * kTileRows + g + 8 * (i / 2);
-                    reinterpret_cast<T*>(a.out + (row0 + xrow) * a.out_stride)[col] = H::round(y);
-                }
-            }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&sh.done_bar[b]));
+        if (++slot == a.stages) {
+            slot = 0;
+            lap ^= 1;
+        }
+    }
+    if (!ok) {
+        // a load that never came, or sums that nobody added: the results are NaN
+        for (long long u = begin + warp; u < end; u += kWarps) {
+            const Run r = run_at(sh, a, u, u + 1, tiles);
+            const int2 x = rows_of(r);
+            const int cols = GATED ? 8 : kTileRows;
+            for (int i = lane; i < x.y * cols; i += 32)
+                reinterpret_cast<T*>(a.out + (x.x + i / cols) * a.out_stride)[r.tile * cols + i % cols] = H::round(__int_as_float(0x7fc00000));
         }
     }
 }

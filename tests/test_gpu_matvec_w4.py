@@ -26,9 +26,11 @@ def expect(x, w, gated):
 
     A product code * x is exact.  The sum: two matrix instructions of 16 products each per 32 columns, each addition off by
     at most a step of fp32 of the terms' magnitude so far; then one product with the scale and one fused addition per 32
-    columns, of which a warp adds up at most 16, and at most 16 warps' sums."""
+    columns, of which a warp adds up at most 16, and at most 16 warps' sums.  By integers the sum is exact but x is not: its
+    31-bit numbers are off by up to half of 2^-30 of the power of two above the row's largest value."""
     y, mag = x.double() @ w.t(), x.double().abs() @ w.abs().t()
     err = (34 * 2.0 ** -23 + (2 * 16 + 16) * 2.0 ** -24) * mag
+    err = err + 2.0 ** -31 * 2 * x.double().abs().amax(1, keepdim=True) * w.abs().sum(1)[None, :]
     if not gated:
         return y, err
     n = w.shape[0] // 2
@@ -144,6 +146,31 @@ def test_infinities_and_nan_stay_in_their_row(pkg):
     hit = w[:, 7]
     assert torch.equal(got[2][hit != 0].double(), torch.sign(hit[hit != 0]) * float("inf")) and got[2][hit == 0].isnan().all()
     assert got[9].isnan().all()
+
+
+@pytest.mark.parametrize("M", [1, 2, 3, 4, 6])
+@pytest.mark.parametrize("zeros", [False, True])
+def test_rows_of_any_magnitude(pkg, M, zeros):
+    """Outliers, rows of zeros, subnormal rows, rows near the end of the range, single values."""
+    N, K = 64, 2048
+    for dtype, scales_of in ((torch.bfloat16, (1.0, 2.0 ** -130, 2.0 ** -100, 2.0 ** 112, 0.0)),
+                             (torch.float16, (1.0, 2.0 ** -22, 2.0 ** -14, 2.0 ** 6, 0.0))):
+        codes, scales, z = make_weights((), N, K, 128, dtype, zeros, M)
+        w = decoded(codes, scales, z)
+        for scale in scales_of:
+            x = torch.randn(M, K, generator=torch.Generator(device="cuda").manual_seed(M), device="cuda").double()
+            x[0, 5] *= 2.0 ** 10          # an outlier
+            x[-1, :1024] *= 2.0 ** -9     # a warp's columns are not another one's
+            x = (x * scale).to(dtype)
+            want, bound = expect(x, w, False)
+            assert close(pkg.matvec_w4(x, codes, scales, zeros=z), want, bound, dtype), (dtype, scale)
+        x = torch.zeros(M, K, dtype=dtype, device="cuda")
+        x[:, 77] = torch.finfo(dtype).max
+        x[:, 78] = torch.finfo(dtype).smallest_normal
+        small = (scales.double() * 2.0 ** -9).to(dtype)   # rounded in fp16, where it is subnormal
+        got = pkg.matvec_w4(x, codes, small, zeros=z)
+        want, bound = expect(x, decoded(codes, small, z), False)
+        assert close(got, want, bound, dtype)
 
 
 def test_a_gate_far_from_zero(pkg):
