@@ -100,8 +100,9 @@ constexpr int kStageInfos = 8;
 
 struct Shared {
     int abort;
-    int warp_sum[kThreads / 32];
+    int2 warp_sum[kThreads / 32];
     int first[kMaxExperts + 1];                // tiles of x rows in front of expert e
+    int cost[kMaxExperts + 1];                 // and what they cost
     alignas(8) uint64_t full_bar[kMaxStages];  // a stage's bytes are there
     alignas(8) uint64_t empty_bar[kMaxStages]; // all multiplying warps have read it
     alignas(8) uint64_t done_bar[2];           // their partial sums are there, in the buffer of the stage's parity
@@ -112,14 +113,35 @@ struct Shared {
 
 // Work is laid out expert by expert.  An expert with more than eight rows meets its weights once per eight of them, in
 // chunks of kChunkTiles tiles, so that the second read of a chunk finds it in L2 (148 CTAs x 8 tiles x 57 KB = 68 MB).
-__device__ __forceinline__ Run run_at(const Shared& sh, const MatvecArgs& a, long long unit, long long end, int tiles)
-{
-    const int at = (int)(unit / tiles);
-    int lo = 0, hi = a.E - 1;   // last expert with first[e] <= at
+__device__ __forceinline__ int last_at_or_below(const int* sums, int n, long long at) {
+    int lo = 0, hi = n - 1;
     while (lo < hi) {
         const int mid = (lo + hi + 1) / 2;
-        if (sh.first[mid] <= at) lo = mid; else hi = mid - 1;
+        if (sums[mid] <= at) lo = mid; else hi = mid - 1;
     }
+    return lo;
+}
+
+// Tiles of up to eight rows, and what they cost: five to eight rows, in the type itself, take the SM a quarter longer than the
+// stream of their weights.
+__device__ __forceinline__ int2 x_tiles_of(int rows) {
+    const int full = rows / kRowsOfX, rest = rows % kRowsOfX;
+    return make_int2(full + (rest > 0), full * 5 + (rest > kFewRows ? 5 : rest > 0 ? 4 : 0));
+}
+
+// First unit (a tile of weights for a tile of x rows, in Run's order) of CTA `share`: the CTAs get equal costs.
+__device__ __forceinline__ long long unit_at_share(const Shared& sh, const MatvecArgs& a, unsigned share, int tiles)
+{
+    const long long all = (long long)sh.cost[a.E] * tiles, at = all * share / gridDim.x;
+    if (share == gridDim.x || all == 0) return (long long)sh.first[a.E] * tiles;
+    const int e = last_at_or_below(sh.cost, a.E, at / tiles);
+    const int x_tiles = sh.first[e + 1] - sh.first[e], cost = sh.cost[e + 1] - sh.cost[e];
+    return (long long)sh.first[e] * tiles + (at - (long long)sh.cost[e] * tiles) * x_tiles / cost;
+}
+
+__device__ __forceinline__ Run run_at(const Shared& sh, const MatvecArgs& a, long long unit, long long end, int tiles)
+{
+    const int lo = last_at_or_below(sh.first, a.E, unit / tiles);
     const int x_tiles = sh.first[lo + 1] - sh.first[lo];
     const long long within = unit - (long long)sh.first[lo] * tiles;
     const int chunk_tiles = x_tiles == 1 ? tiles : kChunkTiles;
@@ -499,43 +521,53 @@ __global__ void __launch_bounds__(kThreads, 1) matvec4_kernel(const MatvecArgs a
     __syncthreads();
     pdl_wait();
 
-    // tiles of x rows per expert, summed up
+    // tiles of x rows per expert and their costs, summed up
     if (a.expert_count) {
-        int run = 0;
+        int2 before = {0, 0};
         for (int e0 = 0; e0 < a.E; e0 += kThreads) {
-            const int e = e0 + threadIdx.x;
-            int n = 0;
+            const int e = e0 + threadIdx.x, sums = min(kThreads, a.E - e0 + 31) / 32;
+            int2 own = {0, 0};
             if (e < a.E) {
                 const int off = a.expert_offset[e], count = a.expert_count[e];
-                if (off >= 0 && count > 0 && off < a.rows) n = (min(count, a.rows - off) + kRowsOfX - 1) / kRowsOfX;
+                if (off >= 0 && count > 0 && off < a.rows) own = x_tiles_of(min(count, a.rows - off));
             }
-            int upto = n;
+            int2 upto = own;
 #pragma unroll
             for (int d = 1; d < 32; d <<= 1) {
-                const int v = __shfl_up_sync(~0u, upto, d);
-                if (lane >= d) upto += v;
+                const int x = __shfl_up_sync(~0u, upto.x, d), y = __shfl_up_sync(~0u, upto.y, d);
+                if (lane >= d) upto.x += x, upto.y += y;
             }
             if (lane == 31) sh.warp_sum[warp] = upto;
             __syncthreads();
-            int total = 0;
-            for (int w = 0; w < kThreads / 32; ++w) {
-                if (w < warp) upto += sh.warp_sum[w];
-                total += sh.warp_sum[w];
+            int2 total = before;
+            for (int w = 0; w < sums; ++w) {
+                const int2 v = sh.warp_sum[w];
+                if (w < warp) upto.x += v.x, upto.y += v.y;
+                total.x += v.x, total.y += v.y;
             }
-            if (e < a.E) sh.first[e] = run + upto - n;
-            run += total;
+            if (e < a.E) {
+                sh.first[e] = before.x + upto.x - own.x;
+                sh.cost[e] = before.y + upto.y - own.y;
+            }
+            before = total;
+            if (e == a.E - 1) {
+                sh.first[a.E] = total.x;
+                sh.cost[a.E] = total.y;
+            }
             __syncthreads();
         }
-        if (threadIdx.x == 0) sh.first[a.E] = run;
-    } else if (threadIdx.x == 0) {
-        sh.first[0] = 0;
-        sh.first[1] = (a.rows + kRowsOfX - 1) / kRowsOfX;
+    } else {
+        if (threadIdx.x == 0) {
+            const int2 v = x_tiles_of(a.rows);
+            sh.first[0] = sh.cost[0] = 0;
+            sh.first[1] = v.x;
+            sh.cost[1] = v.y;
+        }
+        __syncthreads();
     }
-    __syncthreads();
 
     const int tiles = a.N / kTileRows, per_stage = kWarps / a.split, groups = a.K >> (5 + a.group_shift);
-    const long long units = (long long)sh.first[a.E] * tiles;
-    const long long begin = units * blockIdx.x / gridDim.x, end = units * (blockIdx.x + 1) / gridDim.x;
+    const long long begin = unit_at_share(sh, a, blockIdx.x, tiles), end = unit_at_share(sh, a, blockIdx.x + 1, tiles);
 
     // The rows of x and out that a run's tiles meet.
     auto rows_of = [&](const Run& r) {
@@ -675,22 +707,33 @@ __global__ void __launch_bounds__(kThreads, 1) matvec4_kernel(const MatvecArgs a
     // by integers, half of the power of two above the largest value of rows t / 2 and 2 + t / 2 of x; else see load_values
     float unit[2] = {0.0f, 0.0f};
     int slot = 0, lap = 0, row = -1;
-    for (int it = 0;; ++it) {
-        ok = mbar_wait(smem_u32(&sh.full_bar[slot]), lap, &sh.abort);
-        if (!ok) break;
-        const StageInfo s = sh.info[it % kStageInfos];
-        const int b = it & 1;
-        if (s.tiles == 0) {
-            // the adding warps see the end, too; not before all have arrived for the stage two before it
-            if (it >= 2) ok = mbar_wait(smem_u32(&sh.free_bar[b]), (it >> 1) - 1 & 1, &sh.abort);
-            if (ok && lane == 0) mbar_arrive(smem_u32(&sh.done_bar[b]));
-            break;
-        }
-        if (s.row != row) {
-            row = s.row;
+    int2 next = {-1, 0};               // rows of x to take up: at first those of the first run, while its weights are on their way
+    if (begin < end) next = rows_of(run_at(sh, a, begin, end, tiles));
+    StageInfo s = {};
+    bool arrived = false;
+    for (int it = 0;;) {
+        if (next.x != row) {
+            row = next.x;
             form = 0;
-            if (s.rows <= kFewRows) form = load_digits<T>(xr, unit, a, row, s.rows, member, lane);
-            if (form == 0) load_values<T>(xr, unit, a, row, s.rows, member, lane);
+            if (next.y <= kFewRows) form = load_digits<T>(xr, unit, a, row, next.y, member, lane);
+            if (form == 0) load_values<T>(xr, unit, a, row, next.y, member, lane);
+        }
+        const int b = it & 1;
+        if (!arrived) {
+            ok = mbar_wait(smem_u32(&sh.full_bar[slot]), lap, &sh.abort);
+            if (!ok) break;
+            s = sh.info[it % kStageInfos];
+            if (s.tiles == 0) {
+                // the adding warps see the end, too; not before all have arrived for the stage two before it
+                if (it >= 2) ok = mbar_wait(smem_u32(&sh.free_bar[b]), (it >> 1) - 1 & 1, &sh.abort);
+                if (ok && lane == 0) mbar_arrive(smem_u32(&sh.done_bar[b]));
+                break;
+            }
+            arrived = true;
+            if (s.row != row) {
+                next = {s.row, s.rows};
+                continue;
+            }
         }
         float acc[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
         if (of_stage < s.tiles) {
@@ -733,6 +776,8 @@ __global__ void __launch_bounds__(kThreads, 1) matvec4_kernel(const MatvecArgs a
             slot = 0;
             lap ^= 1;
         }
+        ++it;
+        arrived = false;
     }
     if (!ok) {
         // a load that never came, or sums that nobody added: the results are NaN
