@@ -72,6 +72,8 @@ struct MatvecArgs {
     int E, N, K, group_shift;  // group = 32 << group_shift columns
     const int *expert_offset, *expert_count, *row_pair;   // null: one matrix, `rows` rows
     int rows;                  // rows of out
+    unsigned share_step;       // 2^32 / CTAs
+    int prefetch;              // x is small enough to be asked into L2 first
     int split, stages;         // warps that share a tile; ring
     // A stage: the codes of 16 / split tiles, then their scales, then their zero points.  A tile's codes are `chunks` pieces of
     // 128 bytes (256 columns) of its sixteen rows, in the 128-byte swizzle (16-byte unit index XOR row mod 8).
@@ -101,8 +103,6 @@ constexpr int kStageInfos = 8;
 struct Shared {
     int abort;
     int2 warp_sum[kThreads / 32];
-    int first[kMaxExperts + 1];                // tiles of x rows in front of expert e
-    int cost[kMaxExperts + 1];                 // and what they cost
     alignas(8) uint64_t full_bar[kMaxStages];  // a stage's bytes are there
     alignas(8) uint64_t empty_bar[kMaxStages]; // all multiplying warps have read it
     alignas(8) uint64_t done_bar[2];           // their partial sums are there, in the buffer of the stage's parity
@@ -111,49 +111,63 @@ struct Shared {
     alignas(16) float part[2][kWarps][128];
 };
 
-// Work is laid out expert by expert.  An expert with more than eight rows meets its weights once per eight of them, in
-// chunks of kChunkTiles tiles, so that the second read of a chunk finds it in L2 (148 CTAs x 8 tiles x 57 KB = 68 MB).
-__device__ __forceinline__ int last_at_or_below(const int* sums, int n, long long at) {
+// What the CTAs know of the experts' rows, behind the ring: [E + 1] each.
+struct Experts {
+    int* first;    // tiles of x rows in front of expert e
+    int* cost;     // and what they cost
+    int2* rows;    // its first row, and how many
+};
+size_t experts_bytes(int E) { return ((size_t)(E + 1) * 16 + 127) / 128 * 128; }
+
+__device__ __forceinline__ int last_at_or_below(const int* sums, int n, unsigned at) {
     int lo = 0, hi = n - 1;
     while (lo < hi) {
         const int mid = (lo + hi + 1) / 2;
-        if (sums[mid] <= at) lo = mid; else hi = mid - 1;
+        if ((unsigned)sums[mid] <= at) lo = mid; else hi = mid - 1;
     }
     return lo;
 }
 
 // Tiles of up to eight rows, and what they cost: five to eight rows, in the type itself, take the SM a quarter longer than the
 // stream of their weights.
-__device__ __forceinline__ int2 x_tiles_of(int rows) {
+constexpr int kFewCost = 4, kManyCost = 5;
+__host__ __device__ __forceinline__ int2 x_tiles_of(int rows) {
     const int full = rows / kRowsOfX, rest = rows % kRowsOfX;
-    return make_int2(full + (rest > 0), full * 5 + (rest > kFewRows ? 5 : rest > 0 ? 4 : 0));
+    int2 v;
+    v.x = full + (rest > 0);
+    v.y = full * kManyCost + (rest > kFewRows ? kManyCost : rest > 0 ? kFewCost : 0);
+    return v;
 }
 
-// First unit (a tile of weights for a tile of x rows, in Run's order) of CTA `share`: the CTAs get equal costs.
-__device__ __forceinline__ long long unit_at_share(const Shared& sh, const MatvecArgs& a, unsigned share, int tiles)
+// First unit (a tile of weights for a tile of x rows, in Run's order) of CTA `share`: the CTAs get equal costs.  The host sees
+// to it that costs times tiles fit into 32 bits; a 64-bit division would take a microsecond here.
+__device__ __forceinline__ unsigned unit_at_share(const Experts& ex, const MatvecArgs& a, unsigned share, unsigned tiles)
 {
-    const long long all = (long long)sh.cost[a.E] * tiles, at = all * share / gridDim.x;
-    if (share == gridDim.x || all == 0) return (long long)sh.first[a.E] * tiles;
-    const int e = last_at_or_below(sh.cost, a.E, at / tiles);
-    const int x_tiles = sh.first[e + 1] - sh.first[e], cost = sh.cost[e + 1] - sh.cost[e];
-    return (long long)sh.first[e] * tiles + (at - (long long)sh.cost[e] * tiles) * x_tiles / cost;
+    const unsigned all = (unsigned)ex.cost[a.E] * tiles;
+    if (share == gridDim.x || all == 0) return (unsigned)ex.first[a.E] * tiles;
+    const unsigned at = __umulhi(all, share * a.share_step);
+    const int e = last_at_or_below(ex.cost, a.E, at / tiles);
+    const unsigned x_tiles = ex.first[e + 1] - ex.first[e], cost = ex.cost[e + 1] - ex.cost[e], rel = at - (unsigned)ex.cost[e] * tiles;
+    const unsigned unit = x_tiles == 1 ? rel / cost : (unsigned)((unsigned long long)rel * x_tiles / cost);
+    return (unsigned)ex.first[e] * tiles + unit;
 }
 
-__device__ __forceinline__ Run run_at(const Shared& sh, const MatvecArgs& a, long long unit, long long end, int tiles)
+// Work is laid out expert by expert.  An expert with more than eight rows meets its weights once per eight of them, in
+// chunks of kChunkTiles tiles, so that the second read of a chunk finds it in L2 (148 CTAs x 8 tiles x 57 KB = 68 MB).
+__device__ __forceinline__ Run run_at(const Experts& ex, const MatvecArgs& a, unsigned unit, unsigned end, int tiles)
 {
-    const int lo = last_at_or_below(sh.first, a.E, unit / tiles);
-    const int x_tiles = sh.first[lo + 1] - sh.first[lo];
-    const long long within = unit - (long long)sh.first[lo] * tiles;
-    const int chunk_tiles = x_tiles == 1 ? tiles : kChunkTiles;
-    const long long chunk_units = (long long)chunk_tiles * x_tiles;
-    const int chunk = (int)(within / chunk_units), rem = (int)(within - chunk * chunk_units);
-    const int here = min(chunk_tiles, tiles - chunk * chunk_tiles);
-    Run r;
-    r.expert = lo;
-    r.x_tile = rem / here;
-    r.tile = chunk * chunk_tiles + rem % here;
-    r.count = (int)min((long long)(here - rem % here), end - unit);
-    return r;
+    const int e = last_at_or_below(ex.first, a.E, unit / tiles);
+    const int x_tiles = ex.first[e + 1] - ex.first[e], within = unit - ex.first[e] * tiles;
+    if (x_tiles == 1) return {e, 0, within, (int)min((unsigned)(tiles - within), end - unit)};
+    const int chunk = within / (kChunkTiles * x_tiles), rem = within - chunk * kChunkTiles * x_tiles;
+    const int here = min(kChunkTiles, tiles - chunk * kChunkTiles), x_tile = rem / here;
+    return {e, x_tile, chunk * kChunkTiles + rem - x_tile * here, (int)min((unsigned)(here - (rem - x_tile * here)), end - unit)};
+}
+
+// The rows of x and out that a run's tiles meet.
+__device__ __forceinline__ int2 rows_of(const Experts& ex, const Run& r) {
+    const int2 rows = ex.rows[r.expert];
+    return make_int2(rows.x + r.x_tile * kRowsOfX, min(kRowsOfX, rows.y - r.x_tile * kRowsOfX));
 }
 
 __device__ __forceinline__ void box_load_5d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int row, int half, int chunk,
@@ -391,7 +405,15 @@ __device__ __forceinline__ const uint8_t* x_row(const MatvecArgs& a, int row, in
     int src = row + min(i, rows - 1);
     if (a.by_token) src = a.row_pair[src] / a.top_k;
     src = min(max(src, 0), a.x_rows - 1);
-    return a.x + src * a.x_stride + member * 128;
+    return a.x + src * a.x_stride + (member * 64 < a.K ? member * 128 : 0);
+}
+
+// Block j of a warp exists, and its place behind the warp's first one (one that does not exist: the first one's).
+__device__ __forceinline__ bool block_exists(const MatvecArgs& a, int member, int j) {
+    return (2 * (member + j / 2 * a.split) + j % 2) * 32 < a.K;
+}
+__device__ __forceinline__ int x_block(const MatvecArgs& a, int member, int j) {
+    return block_exists(a, member, j) ? j / 2 * a.split * 128 + j % 2 * 64 : 0;
 }
 
 // x for the products in its own type: thread (g, t) holds row g's columns 8t .. 8t+7 of each of its warp's blocks, as the pairs
@@ -403,24 +425,29 @@ __device__ __forceinline__ void load_values(uint32_t (&xr)[kMaxBlocks][4], float
 {
     const int g = lane / 4, t = lane % 4;
     const uint8_t* xp = x_row(a, row, rows, g, member) + 16 * t;
+    if (a.x_wide) {
+        // without a branch, so that all are under way together
+#pragma unroll
+        for (int j = 0; j < kMaxBlocks; ++j) {
+            const uint4 v = *reinterpret_cast<const uint4*>(xp + x_block(a, member, j));
+            xr[j][0] = v.x, xr[j][1] = v.y, xr[j][2] = v.z, xr[j][3] = v.w;
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < kMaxBlocks; ++j) {
+            const uint16_t* h = reinterpret_cast<const uint16_t*>(xp + x_block(a, member, j));
+#pragma unroll
+            for (int i = 0; i < 4; ++i) xr[j][i] = (uint32_t)h[2 * i] | ((uint32_t)h[2 * i + 1] << 16);
+        }
+    }
 #pragma unroll
     for (int j = 0; j < kMaxBlocks; ++j) {
-        uint32_t v[4] = {0, 0, 0, 0};
-        const int block = 2 * (member + j / 2 * a.split) + j % 2, at = (block - 2 * member) * 64;
-        if (block * 32 < a.K) {
-            if (a.x_wide) {
-                const uint4 q = *reinterpret_cast<const uint4*>(xp + at);
-                v[0] = q.x; v[1] = q.y; v[2] = q.z; v[3] = q.w;
-            } else {
-                const uint16_t* h = reinterpret_cast<const uint16_t*>(xp + at);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) v[i] = (uint32_t)h[2 * i] | ((uint32_t)h[2 * i + 1] << 16);
-            }
-        }
-        xr[j][0] = __byte_perm(v[0], v[2], 0x5410);
-        xr[j][1] = __byte_perm(v[0], v[2], 0x7632);
-        xr[j][2] = __byte_perm(v[1], v[3], 0x5410);
-        xr[j][3] = __byte_perm(v[1], v[3], 0x7632);
+        const bool there = block_exists(a, member, j);
+        const uint32_t v0 = there ? xr[j][0] : 0, v1 = there ? xr[j][1] : 0, v2 = there ? xr[j][2] : 0, v3 = there ? xr[j][3] : 0;
+        xr[j][0] = __byte_perm(v0, v2, 0x5410);
+        xr[j][1] = __byte_perm(v0, v2, 0x7632);
+        xr[j][2] = __byte_perm(v1, v3, 0x5410);
+        xr[j][3] = __byte_perm(v1, v3, 0x7632);
     }
     unit[0] = unit[1] = 1.0f;
     if constexpr (Half2<T>::kMantissa == 7) {
@@ -461,21 +488,21 @@ __device__ __forceinline__ int load_digits(uint32_t (&xr)[kMaxBlocks][4], float 
         if (m >= forms) break;
         const uint8_t* xp = x_row(a, row, rows, 2 * m + lane / 16, member) + 16 * t + 4 * q;
         uint32_t raw[kMaxBlocks], most = 0;
+        if (a.x_wide) {
 #pragma unroll
-        for (int j = 0; j < kMaxBlocks; ++j) {
-            const int block = 2 * (member + j / 2 * a.split) + j % 2, at = (block - 2 * member) * 64;
-            raw[j] = 0;
-            if (block * 32 < a.K) {
-                if (a.x_wide) {
-                    raw[j] = *reinterpret_cast<const uint32_t*>(xp + at);
-                } else {
-                    const uint16_t* h = reinterpret_cast<const uint16_t*>(xp + at);
-                    raw[j] = (uint32_t)h[0] | ((uint32_t)h[1] << 16);
-                }
+            for (int j = 0; j < kMaxBlocks; ++j) raw[j] = *reinterpret_cast<const uint32_t*>(xp + x_block(a, member, j));
+        } else {
+#pragma unroll
+            for (int j = 0; j < kMaxBlocks; ++j) {
+                const uint16_t* h = reinterpret_cast<const uint16_t*>(xp + x_block(a, member, j));
+                raw[j] = (uint32_t)h[0] | ((uint32_t)h[1] << 16);
             }
         }
 #pragma unroll
-        for (int j = 0; j < kMaxBlocks; ++j) most = max(most, max(raw[j] & 0x7fffu, raw[j] >> 16 & 0x7fffu));
+        for (int j = 0; j < kMaxBlocks; ++j) {
+            if (!block_exists(a, member, j)) raw[j] = 0;
+            most = max(most, max(raw[j] & 0x7fffu, raw[j] >> 16 & 0x7fffu));
+        }
 #pragma unroll
         for (int d = 1; d < 16; d <<= 1) most = max(most, __shfl_xor_sync(~0u, most, d));
         if (__any_sync(~0u, most >= Half2<T>::kInf)) return 0;
@@ -505,6 +532,10 @@ __global__ void __launch_bounds__(kThreads, 1) matvec4_kernel(const MatvecArgs a
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     uint8_t* const ring = pool + (0u - smem_u32(pool)) % kSwizzleAtom;
     const uint32_t ring0 = smem_u32(ring);
+    Experts ex;
+    ex.rows = reinterpret_cast<int2*>(ring + a.stages * a.stage_bytes);
+    ex.first = reinterpret_cast<int*>(ex.rows + a.E + 1);
+    ex.cost = ex.first + a.E + 1;
     pdl_launch_dependents();
     if (threadIdx.x == 0) {
         sh.abort = 0;
@@ -521,6 +552,19 @@ __global__ void __launch_bounds__(kThreads, 1) matvec4_kernel(const MatvecArgs a
     __syncthreads();
     pdl_wait();
 
+    int2 mine = {0, 0};   // first row and rows of expert threadIdx.x
+    if (a.expert_count && threadIdx.x < a.E) mine = make_int2(a.expert_offset[threadIdx.x], a.expert_count[threadIdx.x]);
+    // x is asked into L2 while these come
+    if (a.prefetch) {
+        const int lines = (a.K * 2 + 127) / 128 + 1, all = a.x_rows * lines;
+        for (int i = blockIdx.x * kThreads + threadIdx.x; i < all; i += gridDim.x * kThreads) {
+            const int r = i / lines, at = min((i - r * lines) * 128, a.K * 2 - 1);
+            prefetch_l2(a.x + r * a.x_stride + at);
+        }
+        if (a.by_token)
+            for (int i = blockIdx.x * kThreads + threadIdx.x; i < (a.rows + 31) / 32; i += gridDim.x * kThreads) prefetch_l2(a.row_pair + i * 32);
+    }
+
     // tiles of x rows per expert and their costs, summed up
     if (a.expert_count) {
         int2 before = {0, 0};
@@ -528,8 +572,10 @@ __global__ void __launch_bounds__(kThreads, 1) matvec4_kernel(const MatvecArgs a
             const int e = e0 + threadIdx.x, sums = min(kThreads, a.E - e0 + 31) / 32;
             int2 own = {0, 0};
             if (e < a.E) {
-                const int off = a.expert_offset[e], count = a.expert_count[e];
-                if (off >= 0 && count > 0 && off < a.rows) own = x_tiles_of(min(count, a.rows - off));
+                const int off = e0 ? a.expert_offset[e] : mine.x, count = e0 ? a.expert_count[e] : mine.y;
+                const int2 rows = off >= 0 && count > 0 && off < a.rows ? make_int2(off, min(count, a.rows - off)) : make_int2(0, 0);
+                own = x_tiles_of(rows.y);
+                ex.rows[e] = rows;
             }
             int2 upto = own;
 #pragma unroll
@@ -546,38 +592,29 @@ __global__ void __launch_bounds__(kThreads, 1) matvec4_kernel(const MatvecArgs a
                 total.x += v.x, total.y += v.y;
             }
             if (e < a.E) {
-                sh.first[e] = before.x + upto.x - own.x;
-                sh.cost[e] = before.y + upto.y - own.y;
+                ex.first[e] = before.x + upto.x - own.x;
+                ex.cost[e] = before.y + upto.y - own.y;
             }
             before = total;
             if (e == a.E - 1) {
-                sh.first[a.E] = total.x;
-                sh.cost[a.E] = total.y;
+                ex.first[a.E] = total.x;
+                ex.cost[a.E] = total.y;
             }
             __syncthreads();
         }
     } else {
         if (threadIdx.x == 0) {
             const int2 v = x_tiles_of(a.rows);
-            sh.first[0] = sh.cost[0] = 0;
-            sh.first[1] = v.x;
-            sh.cost[1] = v.y;
+            ex.first[0] = ex.cost[0] = 0;
+            ex.first[1] = v.x;
+            ex.cost[1] = v.y;
+            ex.rows[0] = {0, a.rows};
         }
         __syncthreads();
     }
 
     const int tiles = a.N / kTileRows, per_stage = kWarps / a.split, groups = a.K >> (5 + a.group_shift);
-    const long long begin = unit_at_share(sh, a, blockIdx.x, tiles), end = unit_at_share(sh, a, blockIdx.x + 1, tiles);
-
-    // The rows of x and out that a run's tiles meet.
-    auto rows_of = [&](const Run& r) {
-        int first = 0, count = a.rows;
-        if (a.expert_count) {
-            first = a.expert_offset[r.expert];
-            count = min(a.expert_count[r.expert], a.rows - first);
-        }
-        return make_int2(first + r.x_tile * kRowsOfX, min(kRowsOfX, count - r.x_tile * kRowsOfX));
-    };
+    const unsigned begin = unit_at_share(ex, a, blockIdx.x, tiles), end = unit_at_share(ex, a, blockIdx.x + 1, tiles);
     bool ok = true;
 
     if (warp >= kWarps) {
@@ -594,9 +631,9 @@ __global__ void __launch_bounds__(kThreads, 1) matvec4_kernel(const MatvecArgs a
                     lap ^= 1;
                 }
             };
-            for (long long u = begin; u < end && ok;) {
-                const Run r = run_at(sh, a, u, end, tiles);
-                const int2 x = rows_of(r);
+            for (unsigned u = begin; u < end && ok;) {
+                const Run r = run_at(ex, a, u, end, tiles);
+                const int2 x = rows_of(ex, r);
                 u += r.count;
                 for (int t0 = 0; t0 < r.count; t0 += per_stage, advance()) {
                     ok = it < a.stages || mbar_wait(smem_u32(&sh.empty_bar[slot]), lap ^ 1, &sh.abort);
@@ -708,7 +745,7 @@ __global__ void __launch_bounds__(kThreads, 1) matvec4_kernel(const MatvecArgs a
     float unit[2] = {0.0f, 0.0f};
     int slot = 0, lap = 0, row = -1;
     int2 next = {-1, 0};               // rows of x to take up: at first those of the first run, while its weights are on their way
-    if (begin < end) next = rows_of(run_at(sh, a, begin, end, tiles));
+    if (begin < end) next = rows_of(ex, run_at(ex, a, begin, end, tiles));
     StageInfo s = {};
     bool arrived = false;
     for (int it = 0;;) {
@@ -781,9 +818,9 @@ __global__ void __launch_bounds__(kThreads, 1) matvec4_kernel(const MatvecArgs a
     }
     if (!ok) {
         // a load that never came, or sums that nobody added: the results are NaN
-        for (long long u = begin + warp; u < end; u += kWarps) {
-            const Run r = run_at(sh, a, u, u + 1, tiles);
-            const int2 x = rows_of(r);
+        for (unsigned u = begin + warp; u < end; u += kWarps) {
+            const Run r = run_at(ex, a, u, u + 1, tiles);
+            const int2 x = rows_of(ex, r);
             const int cols = GATED ? 8 : kTileRows;
             for (int i = lane; i < x.y * cols; i += 32)
                 reinterpret_cast<T*>(a.out + (x.x + i / cols) * a.out_stride)[r.tile * cols + i % cols] = H::round(__int_as_float(0x7fc00000));
@@ -801,7 +838,7 @@ namespace {
 template <typename T, bool GATED, bool FINE, bool ZEROS>
 cudaError_t launch_form(const MatvecArgs& a, const MatvecMaps& maps, int sms, cudaStream_t stream)
 {
-    const size_t smem = (size_t)a.stages * a.stage_bytes + kSwizzleAtom;
+    const size_t smem = (size_t)a.stages * a.stage_bytes + experts_bytes(a.E) + kSwizzleAtom;
     const auto kernel = matvec4_kernel<T, GATED, FINE, ZEROS>;
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return e;
@@ -868,6 +905,8 @@ extern "C" int moe_fp8_b200_matvec_w4(const void* x, int64_t x_stride, int by_to
     }
     if (rows < 0) return bad("num_rows %d < 0", num_rows);
     if (rows == 0) return MOE_FP8_B200_OK;
+    if ((rows / kRowsOfX + w->num_experts + 1) * kManyCost * (w->n / kTileRows) >= ((int64_t)1 << 31))
+        return bad("%lld rows by n = %d are too many for a product of a small batch", (long long)rows, w->n);
     int dev = 0, sms = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
@@ -909,6 +948,8 @@ extern "C" int moe_fp8_b200_matvec_w4(const void* x, int64_t x_stride, int by_to
     a.K = w->k;
     a.group_shift = w->group == 32 ? 0 : w->group == 64 ? 1 : 2;
     a.rows = (int)rows;
+    a.share_step = (unsigned)(((uint64_t)1 << 32) / (unsigned)sms);
+    a.prefetch = x_rows * w->k * 2 <= ((int64_t)4 << 20);
     if (plan) {
         a.top_k = plan->top_k;
         a.expert_offset = plan->expert_offset;
@@ -930,7 +971,7 @@ extern "C" int moe_fp8_b200_matvec_w4(const void* x, int64_t x_stride, int by_to
     a.scale_at = per_stage * a.chunks * 2048;
     a.zero_at = (a.scale_at + per_stage * kTileRows * a.scale_bytes + 127) / 128 * 128;
     a.stage_bytes = (a.zero_at + (w->zeros ? per_stage * kTileRows * a.zero_bytes : 0) + 1023) / 1024 * 1024;
-    a.stages = (int)((kSharedLimit - sizeof(Shared) - kSwizzleAtom - 256) / a.stage_bytes);
+    a.stages = (int)((kSharedLimit - sizeof(Shared) - experts_bytes(a.E) - kSwizzleAtom - 256) / a.stage_bytes);
     if (a.stages > kMaxStages) a.stages = kMaxStages;
     MatvecMaps maps = {};
     int r = encode_weights(maps.codes, w->codes, a, gated != 0, w->k / 2, 128, true);
