@@ -8,6 +8,7 @@
 #include <cuda_runtime.h>
 
 #include <cstring>
+#include <type_traits>
 
 #include "call_checks.cuh"
 #include "ptx.cuh"
@@ -75,58 +76,79 @@ __device__ __forceinline__ int expert_of(const Id* ids, int pair, unsigned long 
 
 size_t sort_smem_bytes(int threads, int E) { return sizeof(int) * (size_t)E * (threads / 32 + 4); }
 
-template <typename Id>
-__global__ void __launch_bounds__(kSortThreads) sort_tokens_kernel(const Id* ids, unsigned long long first,
-                                                                   PlanView p)
+// What a CTA knows after the sort (shared memory).
+struct Sorted {
+    int *seen, *mine, *first_row, *pad_begin, *pad_end;
+    __device__ Sorted(int* smem, int E, int warps) {
+        seen = smem;                // [warps][E] pairs of the expert in earlier warps, then in earlier rounds too
+        mine = seen + warps * E;    // [E] pairs in this CTA
+        first_row = mine + E;       // [E] row of this CTA's first pair
+        pad_begin = first_row + E;  // [E] padding rows of the expert
+        pad_end = pad_begin + E;
+    }
+};
+
+// Sorts the pairs with the CTAs of the cluster (one, if the launch has none) and returns the end of the last expert.  The
+// plan's arrays are written if `publish`; LOCAL: a CTA by itself, which also keeps the pairs' rows in `local_row`.
+// The ids of eight rounds are requested together: a warp's loads would otherwise wait for one another (T = 12288 with top 8:
+// 29 us instead of 12).
+template <typename Id, bool LOCAL>
+__device__ __forceinline__ int sort_pairs(const Id* ids, unsigned long long first, const PlanView& p, const Sorted& s, bool publish,
+                                          int* local_row)
 {
-    extern __shared__ int sort_smem[];
+    constexpr int kBatch = 8;
     __shared__ int warp_sum[32];
     const int E = p.E, warps = blockDim.x / 32, warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-    int* seen = sort_smem;              // [warps][E] pairs of the expert in earlier warps, then in earlier rounds too
-    int* mine = seen + warps * E;       // [E] pairs in this CTA
-    int* first_row = mine + E;          // [E] row of this CTA's first pair
-    int* pad_begin = first_row + E;     // [E] padding rows of the expert
-    int* pad_end = pad_begin + E;
-    const unsigned rank = cluster_rank(), ctas = cluster_size();
-    pdl_launch_dependents();
-    for (int i = threadIdx.x; i < warps * E; i += blockDim.x) seen[i] = 0;
-    __syncthreads();
-    pdl_wait();
-
+    const unsigned rank = LOCAL ? 0 : cluster_rank(), ctas = LOCAL ? 1 : cluster_size();
     const int per_cta = (p.pairs + (int)ctas - 1) / (int)ctas;
     const int cta_end = min(p.pairs, ((int)rank + 1) * per_cta);
     const int per_warp = (per_cta + warps * 32 - 1) / (warps * 32) * 32;
     const int begin = min(cta_end, (int)rank * per_cta + warp * per_warp);
     const int end = min(cta_end, begin + per_warp);
-    int* own = seen + warp * E;
-    for (int i = begin + lane; i < end; i += 32) {
-        const int e = expert_of(ids, i, first, E);
-        if (e >= 0) atomicAdd(own + e, 1);
+    int* own = s.seen + warp * E;
+    for (int i0 = begin + lane; i0 < end + lane; i0 += 32 * kBatch) {
+        int x[kBatch];
+#pragma unroll
+        for (int b = 0; b < kBatch; ++b) x[b] = i0 + 32 * b < end ? expert_of(ids, i0 + 32 * b, first, E) : -1;
+#pragma unroll
+        for (int b = 0; b < kBatch; ++b)
+            if (x[b] >= 0) atomicAdd(own + x[b], 1);
     }
     __syncthreads();
     for (int e = threadIdx.x; e < E; e += blockDim.x) {
         int run = 0;
-        for (int w = 0; w < warps; ++w) {
-            const int c = seen[w * E + e];
-            seen[w * E + e] = run;
-            run += c;
+        for (int w0 = 0; w0 < warps; w0 += kBatch) {
+            int c[kBatch];
+#pragma unroll
+            for (int b = 0; b < kBatch; ++b) c[b] = w0 + b < warps ? s.seen[(w0 + b) * E + e] : 0;
+#pragma unroll
+            for (int b = 0; b < kBatch; ++b) {
+                if (w0 + b < warps) s.seen[(w0 + b) * E + e] = run;
+                run += c[b];
+            }
         }
-        mine[e] = run;
+        s.mine[e] = run;
     }
-    cluster_arrive();
-    cluster_wait();
+    if (!LOCAL) {
+        cluster_arrive();
+        cluster_wait();
+    }
     // one thread per expert (the launch has at least E)
     const int e = threadIdx.x;
     int before = 0, all = 0, padded = 0;
     if (e < E) {
-        for (unsigned c = 0; c < ctas; ++c) {
-            const int v = load_cluster(mine + e, c);
-            if (c < rank) before += v;
-            all += v;
+        if (LOCAL) {
+            all = s.mine[e];
+        } else {
+            for (unsigned c = 0; c < ctas; ++c) {
+                const int v = load_cluster(s.mine + e, c);
+                if (c < rank) before += v;
+                all += v;
+            }
         }
         padded = (all + p.align - 1) / p.align * p.align;
     }
-    cluster_arrive();   // this CTA reads no other one's memory any more; the wait stands at the end
+    if (!LOCAL) cluster_arrive();   // this CTA reads no other one's memory any more; the wait stands at the end
     int upto = padded;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
@@ -136,135 +158,191 @@ __global__ void __launch_bounds__(kSortThreads) sort_tokens_kernel(const Id* ids
     if (lane == 31) warp_sum[warp] = upto;
     __syncthreads();
     int total = 0;
-    for (int w = 0; w < warps; ++w) {
+    for (int w = 0; w < (E + 31) / 32; ++w) {
         if (w < warp) upto += warp_sum[w];
         total += warp_sum[w];
     }
     if (e < E) {
         const int offset = upto - padded;
-        first_row[e] = offset + before;
-        pad_begin[e] = offset + all;
-        pad_end[e] = upto;
-        if (rank == 0) {
+        s.first_row[e] = offset + before;
+        s.pad_begin[e] = offset + all;
+        s.pad_end[e] = upto;
+        if (publish && rank == 0) {
             p.expert_offset[e] = offset;
             p.expert_count[e] = all;
         }
     }
-    if (rank == 0 && threadIdx.x == 0) p.expert_offset[E] = total;
+    if (publish && rank == 0 && threadIdx.x == 0) p.expert_offset[E] = total;
     __syncthreads();
 
-    for (int i0 = begin; i0 < end; i0 += 32) {
-        const int i = i0 + lane;
-        const int x = i < end ? expert_of(ids, i, first, E) : -1;
-        const unsigned same = __match_any_sync(~0u, x);
-        const int prior = x >= 0 ? own[x] : 0;
-        __syncwarp();
-        if (x >= 0 && lane == __ffs(same) - 1) own[x] = prior + __popc(same);
-        __syncwarp();
-        if (i < end) {
-            const int row = x >= 0 ? first_row[x] + prior + __popc(same & ((1u << lane) - 1u)) : -1;
-            p.pair_row[i] = row;
-            if (row >= 0) p.row_pair[row] = i;
+    for (int i0 = begin; i0 < end; i0 += 32 * kBatch) {
+        int batch[kBatch];
+#pragma unroll
+        for (int b = 0; b < kBatch; ++b) batch[b] = i0 + 32 * b + lane < end ? expert_of(ids, i0 + 32 * b + lane, first, E) : -1;
+#pragma unroll
+        for (int b = 0; b < kBatch; ++b) {
+            if (i0 + 32 * b >= end) break;
+            const int i = i0 + 32 * b + lane, x = batch[b];
+            const unsigned same = __match_any_sync(~0u, x);
+            const int prior = x >= 0 ? own[x] : 0;
+            __syncwarp();
+            if (x >= 0 && lane == __ffs(same) - 1) own[x] = prior + __popc(same);
+            __syncwarp();
+            if (i < end) {
+                const int row = x >= 0 ? s.first_row[x] + prior + __popc(same & ((1u << lane) - 1u)) : -1;
+                if (LOCAL) local_row[i] = row;
+                if (publish) {
+                    p.pair_row[i] = row;
+                    if (row >= 0) p.row_pair[row] = i;
+                }
+            }
         }
     }
-    const int cluster_warp = (int)rank * warps + warp, cluster_warps = (int)ctas * warps;
-    if (p.align > 1)
-        for (int x = cluster_warp; x < E; x += cluster_warps)
-            for (int r = pad_begin[x] + lane; r < pad_end[x]; r += 32) p.row_pair[r] = -1;
-    for (int r = total + cluster_warp * 32 + lane; r < p.capacity; r += cluster_warps * 32) p.row_pair[r] = -1;
-    cluster_wait();
+    if (publish) {
+        const int cluster_warp = (int)rank * warps + warp, cluster_warps = (int)ctas * warps;
+        if (p.align > 1)
+            for (int x = cluster_warp; x < E; x += cluster_warps)
+                for (int r = s.pad_begin[x] + lane; r < s.pad_end[x]; r += 32) p.row_pair[r] = -1;
+        for (int r = total + cluster_warp * 32 + lane; r < p.capacity; r += cluster_warps * 32) p.row_pair[r] = -1;
+    }
+    if (!LOCAL) cluster_wait();
+    return total;
+}
+
+template <typename Id>
+__global__ void __launch_bounds__(kSortThreads) sort_tokens_kernel(const Id* ids, unsigned long long first, PlanView p)
+{
+    extern __shared__ int sort_smem[];
+    const Sorted s(sort_smem, p.E, blockDim.x / 32);
+    pdl_launch_dependents();
+    for (int i = threadIdx.x; i < (int)blockDim.x / 32 * p.E; i += blockDim.x) s.seen[i] = 0;
+    __syncthreads();
+    pdl_wait();
+    sort_pairs<Id, false>(ids, first, p, s, true, nullptr);
 }
 
 // ---------------------------------------------------------------------------------------
 // Row types: a piece of N elements, 16 bytes where the rows allow it, else one element.
 // ---------------------------------------------------------------------------------------
-template <typename T> __device__ __forceinline__ float to_float(T v);
-template <> __device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
-template <> __device__ __forceinline__ float to_float(__half v) { return __half2float(v); }
-template <> __device__ __forceinline__ float to_float(float v) { return v; }
-template <typename T> __device__ __forceinline__ T from_float(float v);
-template <> __device__ __forceinline__ __nv_bfloat16 from_float(float v) { return __float2bfloat16_rn(v); }
-template <> __device__ __forceinline__ __half from_float(float v) { return __float2half_rn(v); }
-template <> __device__ __forceinline__ float from_float(float v) { return v; }
+// A piece stays in 32-bit words until its elements are used: as elements, eight bf16 values take eight registers (the
+// combine kernel 100 instead of 64, at half the loads in flight).
+template <typename T, int N>
+struct Piece {
+    typedef T Type;
+    static constexpr int kBytes = sizeof(T) * N;
+    static_assert(kBytes == 16 || N == 1, "16 bytes, or one element");
+    typedef typename std::conditional<kBytes == 16, uint4, typename std::conditional<kBytes == 4, uint32_t, uint16_t>::type>::type Raw;
+    Raw raw;
+    __device__ __forceinline__ uint32_t& word(int i) { return reinterpret_cast<uint32_t*>(&raw)[i]; }
+    __device__ __forceinline__ uint32_t word(int i) const { return reinterpret_cast<const uint32_t*>(&raw)[i]; }
+};
+
+__device__ __forceinline__ float low_half(uint32_t w, __nv_bfloat16) { return __uint_as_float(w << 16); }
+__device__ __forceinline__ float high_half(uint32_t w, __nv_bfloat16) { return __uint_as_float(w & 0xffff0000u); }
+__device__ __forceinline__ float low_half(uint32_t w, __half) { return __half2float(__ushort_as_half((unsigned short)w)); }
+__device__ __forceinline__ float high_half(uint32_t w, __half) { return __half2float(__ushort_as_half((unsigned short)(w >> 16))); }
+__device__ __forceinline__ uint32_t pack_halves(float lo, float hi, __nv_bfloat16) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&v);
+}
+__device__ __forceinline__ uint32_t pack_halves(float lo, float hi, __half) {
+    const __half2 v = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&v);
+}
 
 template <typename T, int N>
-struct alignas(sizeof(T) * N) Piece {
-    T v[N];
-};
+__device__ __forceinline__ void unpack(const Piece<T, N>& p, float (&f)[N]) {
+    if constexpr (sizeof(T) == 4) {
+        if constexpr (N == 1) f[0] = __uint_as_float(p.raw);
+        else
+#pragma unroll
+            for (int i = 0; i < N; ++i) f[i] = __uint_as_float(p.word(i));
+    } else if constexpr (N == 1) {
+        f[0] = low_half(p.raw, T{});
+    } else {
+#pragma unroll
+        for (int i = 0; i < N / 2; ++i) {
+            f[2 * i] = low_half(p.word(i), T{});
+            f[2 * i + 1] = high_half(p.word(i), T{});
+        }
+    }
+}
+template <typename T, int N>
+__device__ __forceinline__ void pack(const float (&f)[N], Piece<T, N>& p) {
+    if constexpr (sizeof(T) == 4) {
+        if constexpr (N == 1) p.raw = __float_as_uint(f[0]);
+        else
+#pragma unroll
+            for (int i = 0; i < N; ++i) p.word(i) = __float_as_uint(f[i]);
+    } else if constexpr (N == 1) {
+        p.raw = (uint16_t)pack_halves(f[0], 0.0f, T{});
+    } else {
+#pragma unroll
+        for (int i = 0; i < N / 2; ++i) p.word(i) = pack_halves(f[2 * i], f[2 * i + 1], T{});
+    }
+}
 
 // Plain loads throughout: a kernel may start while the one that writes its inputs still runs (see pdl_wait), which the
 // read-only path does not allow.
 template <typename P>
-__device__ __forceinline__ P load_piece(const uint8_t* row, int i) { return reinterpret_cast<const P*>(row)[i]; }
+__device__ __forceinline__ P load_piece(const uint8_t* row, int i) {
+    P p;
+    p.raw = reinterpret_cast<const typename P::Raw*>(row)[i];
+    return p;
+}
 template <typename P>
-__device__ __forceinline__ void store_piece(uint8_t* row, int i, const P& v) { reinterpret_cast<P*>(row)[i] = v; }
+__device__ __forceinline__ void store_piece(uint8_t* row, int i, const P& v) { reinterpret_cast<typename P::Raw*>(row)[i] = v.raw; }
 
-// What the CTAs behind the tokens' do: CTA i < E writes zeros to the padding rows of expert i (align > 1), the others to the
-// rows behind the last expert (zero_unused).
+// What the CTAs in front of the tokens' do: padding_split of them write zeros to the padding rows of an expert (align > 1), the
+// others to the rows behind the last expert (zero_unused).  In front, since an expert's padding takes longer than a token.
 constexpr int kUnusedCtas = 592;   // four per SM
 struct Fill {
-    int padding_ctas, unused_ctas;
-    int ctas() const { return padding_ctas + unused_ctas; }
+    int padding_split, padding_ctas, unused_ctas;
+    __host__ __device__ int ctas() const { return padding_ctas + unused_ctas; }
 };
+
+// Zeros in rows begin, begin + step ... below end.
+template <typename P>
+__device__ __forceinline__ void zero_rows(const Rows& rows, int pieces, const PlanView& p, int begin, int end, int step)
+{
+    P zero;
+    memset(&zero, 0, sizeof(P));
+    const int threads = blockDim.x * blockDim.y, tid = threadIdx.y * blockDim.x + threadIdx.x;
+    end = min(p.capacity, end);
+    for (int r = max(0, begin); r < end; r += step)
+        for (int i = blockIdx.y * threads + tid; i < pieces; i += gridDim.y * threads) store_piece(rows[r], i, zero);
+}
 
 template <typename P>
 __device__ void fill_rows(const Rows& rows, int pieces, const PlanView& p, const Fill& fill, int cta)
 {
-    int begin, end, step = 1;
     if (cta < fill.padding_ctas) {
-        begin = p.expert_offset[cta] + p.expert_count[cta];
-        end = p.expert_offset[cta + 1];
+        const int e = cta / fill.padding_split;
+        zero_rows<P>(rows, pieces, p, p.expert_offset[e] + p.expert_count[e] + cta % fill.padding_split, p.expert_offset[e + 1],
+                     fill.padding_split);
     } else {
-        begin = p.expert_offset[p.E];
-        end = p.capacity;
-        step = fill.unused_ctas;
+        zero_rows<P>(rows, pieces, p, p.expert_offset[p.E] + cta - fill.padding_ctas, p.capacity, fill.unused_ctas);
     }
-    begin = max(0, begin) + (step > 1 ? cta - fill.padding_ctas : 0);
-    end = min(p.capacity, end);
-    P zero;
-    memset(&zero, 0, sizeof(P));
-    const int threads = blockDim.x * blockDim.y, tid = threadIdx.y * blockDim.x + threadIdx.x;
-    for (int r = begin; r < end; r += step)
-        for (int i = blockIdx.y * threads + tid; i < pieces; i += gridDim.y * threads) store_piece(rows[r], i, zero);
 }
 
 // ---------------------------------------------------------------------------------------
 // Dispatch: a token is read once and stored to each of its rows.  blockDim.y tokens per CTA, blockDim.x threads over
-// the row's pieces; the CTAs behind the tokens' write the padding.
+// the row's pieces.
 // ---------------------------------------------------------------------------------------
 constexpr int kUnroll = 4;
 
-template <typename T, int N>
-__global__ void __launch_bounds__(256) dispatch_rows_kernel(Rows x, Rows rows, int pieces, int token_ctas, Fill fill,
-                                                            PlanView p)
+template <typename P>
+__device__ __forceinline__ void copy_token(const uint8_t* src, const Rows& rows, const int (&row)[kMaxTopK], int K, int pieces, int begin,
+                                           int step)
 {
-    typedef Piece<T, N> P;
-    pdl_launch_dependents();
-    pdl_wait();
-    if ((int)blockIdx.x >= token_ctas) {
-        fill_rows<P>(rows, pieces, p, fill, (int)blockIdx.x - token_ctas);
-        return;
-    }
-    const int t = blockIdx.x * blockDim.y + threadIdx.y;
-    if (t >= p.T) return;
-    const long long pair0 = (long long)t * p.K;
-    int row[kMaxTopK], any = -1;
-#pragma unroll
-    for (int k = 0; k < kMaxTopK; ++k) {
-        row[k] = k < p.K ? row_of_pair(p, pair0 + k) : -1;
-        any = max(any, row[k]);
-    }
-    if (any < 0) return;
-    const uint8_t* src = x[t];
-    const int step = gridDim.y * blockDim.x;
-    for (int i0 = blockIdx.y * blockDim.x + threadIdx.x; i0 < pieces; i0 += step * kUnroll) {
+    for (int i0 = begin; i0 < pieces; i0 += step * kUnroll) {
         P v[kUnroll];
 #pragma unroll
         for (int u = 0; u < kUnroll; ++u)
             if (i0 + u * step < pieces) v[u] = load_piece<P>(src, i0 + u * step);
 #pragma unroll
         for (int k = 0; k < kMaxTopK; ++k) {
-            if (k >= p.K) break;
+            if (k >= K) break;
             if (row[k] < 0) continue;
             uint8_t* dst = rows[row[k]];
 #pragma unroll
@@ -274,13 +352,72 @@ __global__ void __launch_bounds__(256) dispatch_rows_kernel(Rows x, Rows rows, i
     }
 }
 
+template <typename T, int N>
+__global__ void __launch_bounds__(256) dispatch_rows_kernel(Rows x, Rows rows, int pieces, Fill fill, PlanView p)
+{
+    typedef Piece<T, N> P;
+    pdl_launch_dependents();
+    pdl_wait();
+    const int cta = (int)blockIdx.x - fill.ctas();
+    if (cta < 0) {
+        fill_rows<P>(rows, pieces, p, fill, blockIdx.x);
+        return;
+    }
+    const int t = cta * blockDim.y + threadIdx.y;
+    if (t >= p.T) return;
+    const long long pair0 = (long long)t * p.K;
+    int row[kMaxTopK], any = -1;
+#pragma unroll
+    for (int k = 0; k < kMaxTopK; ++k) {
+        row[k] = k < p.K ? row_of_pair(p, pair0 + k) : -1;
+        any = max(any, row[k]);
+    }
+    if (any < 0) return;
+    copy_token<P>(x[t], rows, row, p.K, pieces, blockIdx.y * blockDim.x + threadIdx.x, gridDim.y * blockDim.x);
+}
+
+// A small batch sorted and copied by one kernel: every CTA sorts all pairs for itself, one of them writes the plan.  What
+// a second launch and the wait between the two cost is more than sorting again (one token: 8 us instead of 11; 128
+// tokens: see the rule where it is launched).
+constexpr int kSmallPairs = 1024, kSmallThreads = 256;
+
+template <typename Id, typename T, int N>
+__global__ void __launch_bounds__(kSmallThreads) sort_and_dispatch_kernel(const Id* ids, unsigned long long first, Rows x, Rows rows,
+                                                                          int pieces, Fill fill, PlanView p)
+{
+    typedef Piece<T, N> P;
+    extern __shared__ int sort_smem[];
+    const Sorted s(sort_smem, p.E, kSmallThreads / 32);
+    int* const local_row = s.pad_end + p.E;
+    pdl_launch_dependents();
+    for (int i = threadIdx.x; i < kSmallThreads / 32 * p.E; i += kSmallThreads) s.seen[i] = 0;
+    __syncthreads();
+    pdl_wait();
+    const int total = sort_pairs<Id, true>(ids, first, p, s, blockIdx.x == 0 && blockIdx.y == 0, local_row);
+    __syncthreads();
+    const int cta = (int)blockIdx.x - fill.ctas();
+    if (cta < 0) {
+        if ((int)blockIdx.x < fill.padding_ctas) {
+            const int e = blockIdx.x / fill.padding_split;
+            zero_rows<P>(rows, pieces, p, s.pad_begin[e] + blockIdx.x % fill.padding_split, s.pad_end[e], fill.padding_split);
+        } else {
+            zero_rows<P>(rows, pieces, p, total + blockIdx.x - fill.padding_ctas, p.capacity, fill.unused_ctas);
+        }
+        return;
+    }
+    int row[kMaxTopK];
+#pragma unroll
+    for (int k = 0; k < kMaxTopK; ++k) row[k] = k < p.K ? local_row[cta * p.K + k] : -1;
+    copy_token<P>(x[cta], rows, row, p.K, pieces, blockIdx.y * kSmallThreads + threadIdx.x, gridDim.y * kSmallThreads);
+}
+
 // ---------------------------------------------------------------------------------------
 // Combine: eight rows' pieces of a column are requested together, then added in pair order.
 // ---------------------------------------------------------------------------------------
 constexpr int kRowsAtOnce = 8;
 
 template <typename T, int N, bool WEIGHTED>
-__global__ void __launch_bounds__(256) combine_rows_kernel(Rows y, const float* weights, Rows out, int pieces,
+__global__ void __launch_bounds__(256, 4) combine_rows_kernel(Rows y, const float* weights, Rows out, int pieces,
                                                            PlanView p)
 {
     typedef Piece<T, N> P;
@@ -307,40 +444,41 @@ __global__ void __launch_bounds__(256) combine_rows_kernel(Rows y, const float* 
                 if (row[k] >= 0) v[k] = load_piece<P>(y[row[k]], i);
 #pragma unroll
             for (int k = 0; k < kRowsAtOnce; ++k)
-                if (row[k] >= 0)
+                if (row[k] >= 0) {
+                    float f[N];
+                    unpack(v[k], f);
 #pragma unroll
-                    for (int j = 0; j < N; ++j)
-                        acc[j] = WEIGHTED ? fmaf(to_float(v[k].v[j]), w[k], acc[j]) : acc[j] + to_float(v[k].v[j]);
+                    for (int j = 0; j < N; ++j) acc[j] = WEIGHTED ? fmaf(f[j], w[k], acc[j]) : acc[j] + f[j];
+                }
         }
         P o;
-#pragma unroll
-        for (int j = 0; j < N; ++j) o.v[j] = from_float<T>(acc[j]);
+        pack(acc, o);
         store_piece(out[t], i, o);
     }
 }
 
 // ---------------------------------------------------------------------------------------
-// The combine's gradient: a CTA takes a token, its warps share the token's rows.  A row's warps walk its pieces, scale
-// the token's gradient into the row's gradient and sum the products with the row; the sums meet in shared memory in a
-// fixed order.  The token's gradient is read by every row's warps, out of L1 after the first.
+// The combine's gradient: a CTA takes a token.  A thread reads a piece of the token's gradient once, and with it eight rows'
+// pieces of y: it scales the gradient into those rows' gradients and adds up the products with them.  The sums meet over
+// the warp and in shared memory, in a fixed order.
 // ---------------------------------------------------------------------------------------
-constexpr int kGradWarps = 8;
+constexpr int kGradThreads = 256;
 
 template <typename T, int N>
-__global__ void __launch_bounds__(kGradWarps * 32) combine_grad_kernel(Rows grad_out, Rows y, const float* weights,
-                                                                       Rows grad_y, float* grad_weights,
-                                                                       int pieces, Fill fill, PlanView p)
+__global__ void __launch_bounds__(kGradThreads, 3) combine_grad_kernel(Rows grad_out, Rows y, const float* weights, Rows grad_y,
+                                                                       float* grad_weights, int pieces, Fill fill, PlanView p)
 {
     typedef Piece<T, N> P;
     __shared__ int live_row[kMaxTopK], live_k[kMaxTopK], live_count;
-    __shared__ float part_sum[kGradWarps];
+    __shared__ float part_sum[kRowsAtOnce][kGradThreads / 32];
     pdl_launch_dependents();
     pdl_wait();
-    if ((int)blockIdx.x >= p.T) {
-        fill_rows<P>(grad_y, pieces, p, fill, (int)blockIdx.x - p.T);
+    const int t = (int)blockIdx.x - fill.ctas();
+    if (t < 0) {
+        fill_rows<P>(grad_y, pieces, p, fill, blockIdx.x);
         return;
     }
-    const int t = blockIdx.x, warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, warps = blockDim.x / 32;
     if (warp == 0) {
         const int row = lane < p.K ? row_of_pair(p, (long long)t * p.K + lane) : -1;
         const unsigned live = __ballot_sync(~0u, row >= 0);
@@ -356,45 +494,56 @@ __global__ void __launch_bounds__(kGradWarps * 32) combine_grad_kernel(Rows grad
     __syncthreads();
     const int count = live_count;
     const uint8_t* src = grad_out[t];
-    for (int base = 0; base < count; base += kGradWarps) {
-        // rows base .. base + rows - 1; warps with the same remainder share one
-        const int rows = min(kGradWarps, count - base);
-        const int j = base + warp % rows, part = warp / rows, parts = (kGradWarps - warp % rows + rows - 1) / rows;
-        const float w = weights[(long long)t * p.K + live_k[j]];
-        float sum = 0.0f;
-        for (int i0 = part * 32 + lane; i0 < pieces; i0 += parts * 32 * kUnroll) {
-            P g[kUnroll], v[kUnroll];
+    for (int base = 0; base < count; base += kRowsAtOnce) {
+        const int rows = min(kRowsAtOnce, count - base);
+        int row[kRowsAtOnce];
+        float w[kRowsAtOnce], sum[kRowsAtOnce];
 #pragma unroll
-            for (int u = 0; u < kUnroll; ++u) {
-                const int i = i0 + u * parts * 32;
-                if (i < pieces) {
-                    if (grad_weights) v[u] = load_piece<P>(y[live_row[j]], i);
-                    g[u] = load_piece<P>(src, i);
-                }
+        for (int k = 0; k < kRowsAtOnce; ++k) {
+            row[k] = k < rows ? live_row[base + k] : 0;
+            w[k] = k < rows ? weights[(long long)t * p.K + live_k[base + k]] : 0.0f;
+            sum[k] = 0.0f;
+        }
+        for (int i = threadIdx.x; i < pieces; i += blockDim.x) {
+            const P piece = load_piece<P>(src, i);
+            P v[kRowsAtOnce];
+            if (grad_weights) {
+#pragma unroll
+                for (int k = 0; k < kRowsAtOnce; ++k)
+                    if (k < rows) v[k] = load_piece<P>(y[row[k]], i);
             }
 #pragma unroll
-            for (int u = 0; u < kUnroll; ++u) {
-                const int i = i0 + u * parts * 32;
-                if (i < pieces) {
+            for (int k = 0; k < kRowsAtOnce; ++k) {
+                if (k >= rows) break;
+                float g[N], f[N];
+                unpack(piece, g);
+                if (grad_weights) {
+                    unpack(v[k], f);
+#pragma unroll
+                    for (int n = 0; n < N; ++n) sum[k] = fmaf(g[n], f[n], sum[k]);
+                }
+                if (grad_y.base) {
                     P o;
 #pragma unroll
-                    for (int n = 0; n < N; ++n) {
-                        const float f = to_float(g[u].v[n]);
-                        o.v[n] = from_float<T>(f * w);
-                        if (grad_weights) sum = fmaf(f, to_float(v[u].v[n]), sum);
-                    }
-                    if (grad_y.base) store_piece(grad_y[live_row[j]], i, o);
+                    for (int n = 0; n < N; ++n) f[n] = g[n] * w[k];
+                    pack(f, o);
+                    store_piece(grad_y[row[k]], i, o);
                 }
             }
         }
         if (grad_weights) {
 #pragma unroll
-            for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(~0u, sum, d);
-            if (lane == 0) part_sum[warp] = sum;
+            for (int k = 0; k < kRowsAtOnce; ++k) {
+                if (k >= rows) break;
+                float s = sum[k];
+#pragma unroll
+                for (int d = 16; d > 0; d >>= 1) s += __shfl_xor_sync(~0u, s, d);
+                if (lane == 0) part_sum[k][warp] = s;
+            }
             __syncthreads();
             if ((int)threadIdx.x < rows) {
                 float s = 0.0f;
-                for (int q = threadIdx.x; q < kGradWarps; q += rows) s += part_sum[q];
+                for (int q = 0; q < warps; ++q) s += part_sum[threadIdx.x][q];
                 grad_weights[(long long)t * p.K + live_k[base + threadIdx.x]] = s;
             }
             __syncthreads();
@@ -533,21 +682,47 @@ cudaError_t launch_dispatch(const Extent& x, const Extent& rows, const PlanView&
 {
     const int pieces = (int)(x.row_bytes / (int64_t)(sizeof(T) * N));
     const Shape s = shape_for(p.T, pieces);
-    return launch_after(dispatch_rows_kernel<T, N>, dim3(s.token_ctas + fill.ctas(), s.splits), s.block, 0, 1, stream,
-                        as_rows(x), as_rows(rows), pieces, s.token_ctas, fill, p);
+    return launch_after(dispatch_rows_kernel<T, N>, dim3(fill.ctas() + s.token_ctas, s.splits), s.block, 0, 1, stream, as_rows(x),
+                        as_rows(rows), pieces, fill, p);
 }
 
-Fill fill_for(const PlanView& p, int zero_unused) { return {p.align > 1 ? p.E : 0, zero_unused ? kUnusedCtas : 0}; }
+Fill fill_for(const PlanView& p, int zero_unused)
+{
+    const int split = p.align >= 32 ? 8 : 1;   // an expert's padding is align / 2 rows on average
+    return {split, p.align > 1 ? p.E * split : 0, zero_unused ? kUnusedCtas : 0};
+}
 
-cudaError_t enqueue_dispatch(const Extent& x, const Extent& rows, int dtype, const PlanView& p, int zero_unused,
-                             cudaStream_t stream)
+template <typename Id, typename T, int N>
+cudaError_t launch_small(const void* ids, int64_t first, const Extent& x, const Extent& rows, const PlanView& p, const Fill& fill,
+                         cudaStream_t stream)
+{
+    const int pieces = (int)(x.row_bytes / (int64_t)(sizeof(T) * N));
+    const int passes = (pieces + kSmallThreads - 1) / kSmallThreads;
+    int splits = (148 + p.T - 1) / p.T;
+    if (splits > passes) splits = passes;
+    const size_t smem = sort_smem_bytes(kSmallThreads, p.E) + sizeof(int) * (size_t)p.pairs;
+    return launch_after(sort_and_dispatch_kernel<Id, T, N>, dim3(fill.ctas() + p.T, splits), dim3(kSmallThreads), smem, 1, stream,
+                        static_cast<const Id*>(ids), (unsigned long long)first, as_rows(x), as_rows(rows), pieces, fill, p);
+}
+
+// The copy needs no arithmetic: one form per element size.  `ids`: sorted here first, if the batch is small in the same kernel.
+cudaError_t enqueue_dispatch(const void* ids, int id_bits, int64_t first, const Extent& x, const Extent& rows, int dtype,
+                             const PlanView& p, int zero_unused, cudaStream_t stream)
 {
     const Fill fill = fill_for(p, zero_unused);
-    // the copy needs no arithmetic: one form per element size
     const bool wide = on_16_bytes(x) && on_16_bytes(rows);
+    auto with = [&](auto type, auto n) {
+        typedef decltype(type) T;
+        constexpr int N = decltype(n)::value;
+        if (ids && p.pairs <= kSmallPairs && p.E <= kSmallThreads)
+            return id_bits == 32 ? launch_small<int32_t, T, N>(ids, first, x, rows, p, fill, stream)
+                                 : launch_small<int64_t, T, N>(ids, first, x, rows, p, fill, stream);
+        const cudaError_t e = ids ? enqueue_sort(ids, id_bits, first, p, stream) : cudaSuccess;
+        return e == cudaSuccess ? launch_dispatch<T, N>(x, rows, p, fill, stream) : e;
+    };
     if (element_size(dtype) == 4)
-        return wide ? launch_dispatch<float, 4>(x, rows, p, fill, stream) : launch_dispatch<float, 1>(x, rows, p, fill, stream);
-    return wide ? launch_dispatch<__half, 8>(x, rows, p, fill, stream) : launch_dispatch<__half, 1>(x, rows, p, fill, stream);
+        return wide ? with(float{}, std::integral_constant<int, 4>{}) : with(float{}, std::integral_constant<int, 1>{});
+    return wide ? with(__half{}, std::integral_constant<int, 8>{}) : with(__half{}, std::integral_constant<int, 1>{});
 }
 
 template <typename T, int N>
@@ -564,9 +739,10 @@ cudaError_t launch_combine_grad(const Extent& grad_out, const Extent& y, const f
                                 float* grad_weights, const PlanView& p, int zero_unused, cudaStream_t stream)
 {
     const int pieces = (int)(grad_out.row_bytes / (int64_t)(sizeof(T) * N));
-    const Fill fill = grad_y.base ? fill_for(p, zero_unused) : Fill{0, 0};
-    return launch_after(combine_grad_kernel<T, N>, dim3(p.T + fill.ctas()), dim3(kGradWarps * 32), 0, 1, stream, as_rows(grad_out),
-                        as_rows(y), weights, as_rows(grad_y), grad_weights, pieces, fill, p);
+    const Fill fill = grad_y.base ? fill_for(p, zero_unused) : Fill{1, 0, 0};
+    const int passes = (pieces + kGradThreads - 1) / kGradThreads, threads = ((pieces + passes - 1) / passes + 31) / 32 * 32;
+    return launch_after(combine_grad_kernel<T, N>, dim3(fill.ctas() + p.T), dim3(threads), 0, 1, stream, as_rows(grad_out), as_rows(y),
+                        weights, as_rows(grad_y), grad_weights, pieces, fill, p);
 }
 
 int check_ids(const Call& call, const void* ids, int id_bits)
@@ -610,7 +786,7 @@ int moe_fp8_b200_dispatch_rows(const void* x, int64_t x_stride, void* rows, int6
     if (rc == MOE_FP8_B200_OK) rc = check_rows(call, "rows", rows, rows_stride, p.capacity, dtype, hidden, true, er);
     if (rc == MOE_FP8_B200_OK) rc = check_apart(call, er, ex);
     if (rc != MOE_FP8_B200_OK) return rc;
-    return call.cuda(enqueue_dispatch(ex, er, dtype, p, zero_unused, static_cast<cudaStream_t>(stream)));
+    return call.cuda(enqueue_dispatch(nullptr, 0, 0, ex, er, dtype, p, zero_unused, static_cast<cudaStream_t>(stream)));
 }
 
 int moe_fp8_b200_sort_and_dispatch(const void* topk_idx, int id_bits, int64_t first_expert, const void* x, int64_t x_stride,
@@ -627,9 +803,8 @@ int moe_fp8_b200_sort_and_dispatch(const void* topk_idx, int id_bits, int64_t fi
     if (rc == MOE_FP8_B200_OK && p.T > 0) rc = check_apart(call, er, ex);
     if (rc != MOE_FP8_B200_OK) return rc;
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
-    cudaError_t e = enqueue_sort(topk_idx, id_bits, first_expert, p, s);
-    if (e == cudaSuccess && p.T > 0) e = enqueue_dispatch(ex, er, dtype, p, zero_unused, s);
-    return call.cuda(e);
+    return call.cuda(p.T > 0 ? enqueue_dispatch(topk_idx, id_bits, first_expert, ex, er, dtype, p, zero_unused, s)
+                             : enqueue_sort(topk_idx, id_bits, first_expert, p, s));
 }
 
 int moe_fp8_b200_combine_rows(const void* y, int64_t y_stride, const float* weights, void* out, int64_t out_stride, int dtype,
