@@ -76,6 +76,18 @@ __device__ __forceinline__ int expert_of(const Id* ids, int pair, unsigned long 
 
 size_t sort_smem_bytes(int threads, int E) { return sizeof(int) * (size_t)E * (threads / 32 + 4); }
 
+// The lanes whose x agrees in its low bits.  A vote per bit: nine of them take less time than one match over the warp (98304
+// pairs: 16.4 us, 18.5 with the match).
+__device__ __forceinline__ unsigned lanes_with(int x, int bits) {
+    unsigned same = ~0u;
+    for (int b = 0; b < bits; ++b) {
+        const bool one = x >> b & 1;
+        const unsigned v = __ballot_sync(~0u, one);
+        same &= one ? v : ~v;
+    }
+    return same;
+}
+
 // What a CTA knows after the sort (shared memory).
 struct Sorted {
     int *seen, *mine, *first_row, *pad_begin, *pad_end;
@@ -90,8 +102,7 @@ struct Sorted {
 
 // Sorts the pairs with the CTAs of the cluster (one, if the launch has none) and returns the end of the last expert.  The
 // plan's arrays are written if `publish`; LOCAL: a CTA by itself, which also keeps the pairs' rows in `local_row`.
-// The ids of eight rounds are requested together: a warp's loads would otherwise wait for one another (T = 12288 with top 8:
-// 29 us instead of 12).
+// The ids of eight rounds are requested together, since a warp's loads would otherwise wait for one another.
 template <typename Id, bool LOCAL>
 __device__ __forceinline__ int sort_pairs(const Id* ids, unsigned long long first, const PlanView& p, const Sorted& s, bool publish,
                                           int* local_row)
@@ -106,6 +117,7 @@ __device__ __forceinline__ int sort_pairs(const Id* ids, unsigned long long firs
     const int begin = min(cta_end, (int)rank * per_cta + warp * per_warp);
     const int end = min(cta_end, begin + per_warp);
     int* own = s.seen + warp * E;
+    const int bits = 32 - __clz(E);   // -1 has a pattern of its own among them
     for (int i0 = begin + lane; i0 < end + lane; i0 += 32 * kBatch) {
         int x[kBatch];
 #pragma unroll
@@ -183,7 +195,7 @@ __device__ __forceinline__ int sort_pairs(const Id* ids, unsigned long long firs
         for (int b = 0; b < kBatch; ++b) {
             if (i0 + 32 * b >= end) break;
             const int i = i0 + 32 * b + lane, x = batch[b];
-            const unsigned same = __match_any_sync(~0u, x);
+            const unsigned same = lanes_with(x, bits);
             const int prior = x >= 0 ? own[x] : 0;
             __syncwarp();
             if (x >= 0 && lane == __ffs(same) - 1) own[x] = prior + __popc(same);
@@ -376,10 +388,10 @@ __global__ void __launch_bounds__(256) dispatch_rows_kernel(Rows x, Rows rows, i
     copy_token<P>(x[t], rows, row, p.K, pieces, blockIdx.y * blockDim.x + threadIdx.x, gridDim.y * blockDim.x);
 }
 
-// A small batch sorted and copied by one kernel: every CTA sorts all pairs for itself, one of them writes the plan.  What
-// a second launch and the wait between the two cost is more than sorting again (one token: 8 us instead of 11; 128
-// tokens: see the rule where it is launched).
-constexpr int kSmallPairs = 1024, kSmallThreads = 256;
+// A small batch sorted and copied by one kernel: every CTA sorts all pairs for itself, one of them writes the plan.  Up to 2048
+// pairs that costs less than a second launch and the wait between the two (top 8, 7168 columns, us by one and by two
+// kernels: 1 token 8.2 / 11.3, 128 tokens 13.2 / 17.4, 256 tokens 16.4 / 19.4, 512 tokens 28.7 / 25.6).
+constexpr int kSmallPairs = 2048, kSmallTokens = 256, kSmallThreads = 256;
 
 template <typename Id, typename T, int N>
 __global__ void __launch_bounds__(kSmallThreads) sort_and_dispatch_kernel(const Id* ids, unsigned long long first, Rows x, Rows rows,
@@ -559,7 +571,7 @@ int64_t plan_rows(int64_t T, int64_t K, int64_t E, int64_t align)
     if (T < 0 || K < 1 || K > kMaxTopK || E < 1 || E > kMaxExperts || align < 1 || align > kMaxAlign) return -1;
     const int64_t pairs = T * K, most = pairs + (E < pairs ? E : pairs) * (align - 1);
     const int64_t rows = (most + align - 1) / align * align;
-    return rows <= INT32_MAX - 2 * kSortThreads * 8 ? rows : -1;   // index arithmetic of the sort stays in 32 bits
+    return rows <= INT32_MAX - 2 * kSortThreads * 16 ? rows : -1;   // index arithmetic of the sort stays in 32 bits
 }
 
 struct Call {
@@ -659,8 +671,14 @@ Shape shape_for(int T, int pieces)
 template <typename Id>
 cudaError_t launch_sort(const void* ids, int64_t first, const PlanView& p, cudaStream_t stream)
 {
-    // the cluster grows with the batch: a CTA takes 32 pairs per warp at least
-    const unsigned ctas = p.pairs <= kSortThreads ? 1 : p.pairs <= 2 * kSortThreads ? 2 : p.pairs <= 4 * kSortThreads ? 4 : 8;
+    // The cluster grows with the batch: a CTA takes 32 pairs per warp at least.  Sixteen CTAs (98304 pairs: 16.4 us, 22.5 with
+    // eight) have to be allowed for, and lie within one GPC.
+    unsigned ctas = 1;
+    while (ctas < 16 && p.pairs > (int)ctas * kSortThreads) ctas *= 2;
+    if (ctas == 16) {
+        const cudaError_t e = cudaFuncSetAttribute(sort_tokens_kernel<Id>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+        if (e != cudaSuccess) return e;
+    }
     const int need = p.E > p.pairs ? p.E : p.pairs;
     const int threads = need >= kSortThreads ? kSortThreads : need <= 128 ? 128 : (need + 31) / 32 * 32;
     const size_t smem = sort_smem_bytes(threads, p.E);
@@ -714,7 +732,7 @@ cudaError_t enqueue_dispatch(const void* ids, int id_bits, int64_t first, const 
     auto with = [&](auto type, auto n) {
         typedef decltype(type) T;
         constexpr int N = decltype(n)::value;
-        if (ids && p.pairs <= kSmallPairs && p.E <= kSmallThreads)
+        if (ids && p.pairs <= kSmallPairs && p.T <= kSmallTokens && p.E <= kSmallThreads)
             return id_bits == 32 ? launch_small<int32_t, T, N>(ids, first, x, rows, p, fill, stream)
                                  : launch_small<int64_t, T, N>(ids, first, x, rows, p, fill, stream);
         const cudaError_t e = ids ? enqueue_sort(ids, id_bits, first, p, stream) : cudaSuccess;

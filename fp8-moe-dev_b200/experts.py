@@ -25,6 +25,7 @@ _ROW_TYPES = {torch.bfloat16: _lib.BF16, torch.float16: _lib.FP16, torch.float32
 _ID_BITS = {torch.int32: 32, torch.int64: 64}
 _raw_stream = torch._C._cuda_getCurrentRawStream
 _ERR_BYTES = 256
+_SMALL = 1 << 20   # tokens up to which a plan's size needs no word from the library
 
 
 def _call(fn, device, *args):
@@ -88,7 +89,11 @@ def _row_type(name, t):
 
 def plan_rows(num_tokens: int, top_k: int, num_experts: int, align: int = 1) -> int:
     """Rows that any choice of experts fits into: what `rows` of a dispatch must hold."""
-    rows = _lib.load().moe_fp8_b200_plan_rows(int(num_tokens), int(top_k), int(num_experts), int(align))
+    T, K, E, align = int(num_tokens), int(top_k), int(num_experts), int(align)
+    if 0 <= T <= _SMALL and 1 <= K <= _lib.PLAN_MAX_TOP_K and 1 <= E <= _lib.PLAN_MAX_EXPERTS and 1 <= align <= 1024:
+        pairs = T * K
+        return (pairs + min(E, pairs) * (align - 1) + align - 1) // align * align
+    rows = _lib.load().moe_fp8_b200_plan_rows(T, K, E, align)
     if rows < 0:
         raise ValueError(f"no plan for {num_tokens} tokens, top_k {top_k} (1 .. {_lib.PLAN_MAX_TOP_K}), {num_experts} experts "
                          f"(1 .. {_lib.PLAN_MAX_EXPERTS}), align {align} (1 .. 1024)")
