@@ -69,18 +69,20 @@ struct MatvecArgs {
     const uint8_t* zeros;      // or null: 8
     uint8_t* out;
     long long out_stride;
-    int E, N, K, group_shift;  // group = 32 << group_shift columns
+    int E, N, K, group, gated;
     const int *expert_offset, *expert_count, *row_pair;   // null: one matrix, `rows` rows
     int rows;                  // rows of out
     unsigned share_step;       // 2^32 / CTAs
     int prefetch;              // x is small enough to be asked into L2 first
-    int split, stages;         // warps that share a tile; ring
-    // A stage: the codes of 16 / split tiles, then their scales, then their zero points.  A tile's codes are `chunks` pieces of
+    int stages;                // of the ring
+    // A stage: the codes of 16 / SPLIT tiles, then their scales, then their zero points.  A tile's codes are `chunks` pieces of
     // 128 bytes (256 columns) of its sixteen rows, in the 128-byte swizzle (16-byte unit index XOR row mod 8).
     int chunks, whole;             // whole: a row is a multiple of 128 bytes, one box takes a tile
+    int scale_step;                // scales from a pair of a warp to its next
     int scale_bytes, zero_bytes;   // pitch of a row's scales and zero points
     int scale_box, zero_box;       // they come as boxes, else (rows of no multiple of 16 bytes) as they lie
     int scale_at, zero_at, stage_bytes;
+    unsigned tile_bytes;           // that arrive per tile
 };
 
 // The weights as TMA sees them: gated ones as two halves of n / 2 rows, of which a tile takes the same eight.
@@ -108,6 +110,9 @@ struct Shared {
     alignas(8) uint64_t done_bar[2];           // their partial sums are there, in the buffer of the stage's parity
     alignas(8) uint64_t free_bar[2];           // and have been added up
     alignas(16) StageInfo info[kStageInfos];
+    StageInfo start;                           // the first run's rows, before its weights are there
+    unsigned begin, end;                       // this CTA's units
+    float unit[kWarps][kRowsOfX];              // a multiplying warp's scales of x's rows (see load_digits, load_values)
     alignas(16) float part[2][kWarps][128];
 };
 
@@ -265,29 +270,29 @@ __device__ __forceinline__ uint32_t xor_and(uint32_t a, uint32_t b, uint32_t mas
     return d;
 }
 
-// A thread's part of a tile in shared memory (bytes into the ring).  A warp takes every split-th pair of 32-column blocks,
-// so that its pairs lie at one distance, split / 4 chunks.
+// A thread's part of a tile in shared memory (bytes into the ring).  SPLIT warps share a tile, and each takes every SPLIT-th pair
+// of 32-column blocks: its pairs lie SPLIT / 4 chunks apart.  With SPLIT a constant, so are the distances, and the loads need
+// no arithmetic; registers are what this kernel has least of (a spilled one comes back out of L2, behind the weights).
 struct TileView {
     const uint8_t* ring;
-    int even, odd;     // its word of the first pair's two blocks in weight row g; row g + 8 lies 1024 bytes further
-    int scales, zeros; // its row's scale and zero point of the first pair; row g + 8's lie scale_rows, zero_rows further
-    int scale_rows, zero_rows;
-    int pair_step, scale_step, zero_step;
-    int last_scale, last_zero;   // of the row: a pair's second block may lie behind the last column, where x is zero
+    int even;              // its word of the first pair's first block in weight row g (the second's: ^ 16); row g + 8 lies 1024 bytes further
+    int scales, zeros;     // its row's scale and zero point of the first pair; row g + 8's lie 8 rows further
+    int blocks;            // of the warp; a last pair's second block may not exist (its x is zero)
 };
 
 // The words of COUNT pairs of blocks from `pair` on, and the scales and zero points of one.
-template <int COUNT>
+template <int SPLIT, int COUNT>
 struct Words {
     uint32_t row0[2 * COUNT], row1[2 * COUNT];
     __device__ __forceinline__ Words(const TileView& v, int pair) {
 #pragma unroll
         for (int p = 0; p < COUNT; ++p) {
-            const int at = (pair + p) * v.pair_step;
-            row0[2 * p] = *reinterpret_cast<const uint32_t*>(v.ring + v.even + at);
-            row1[2 * p] = *reinterpret_cast<const uint32_t*>(v.ring + v.even + at + 1024);
-            row0[2 * p + 1] = *reinterpret_cast<const uint32_t*>(v.ring + v.odd + at);
-            row1[2 * p + 1] = *reinterpret_cast<const uint32_t*>(v.ring + v.odd + at + 1024);
+            const uint8_t* at = v.ring + (pair + p) * (SPLIT * 512);
+            const int odd = v.even ^ 16;
+            row0[2 * p] = *reinterpret_cast<const uint32_t*>(at + v.even);
+            row1[2 * p] = *reinterpret_cast<const uint32_t*>(at + v.even + 1024);
+            row0[2 * p + 1] = *reinterpret_cast<const uint32_t*>(at + odd);
+            row1[2 * p + 1] = *reinterpret_cast<const uint32_t*>(at + odd + 1024);
         }
     }
 };
@@ -296,33 +301,31 @@ template <typename H, bool ZEROS>
 struct Scales {
     float s0, s1;
     uint32_t z0, z1;
-    __device__ __forceinline__ Scales(const TileView& v, int pair, bool second) {
-        int sa = v.scales + pair * v.scale_step, za = v.zeros + pair * v.zero_step;
-        if (second) {
-            sa = min(sa + 2, v.last_scale);
-            za = min(za + 1, v.last_zero);
-        }
+    __device__ __forceinline__ Scales(const MatvecArgs& a, const TileView& v, int pair, bool second) {
+        const int sa = v.scales + pair * (2 * a.scale_step) + (second ? 2 : 0), za = v.zeros + pair * a.scale_step + (second ? 1 : 0);
         s0 = H::scale(*reinterpret_cast<const uint16_t*>(v.ring + sa));
-        s1 = H::scale(*reinterpret_cast<const uint16_t*>(v.ring + sa + v.scale_rows));
+        s1 = H::scale(*reinterpret_cast<const uint16_t*>(v.ring + sa + 8 * a.scale_bytes));
         z0 = ZEROS ? v.ring[za] : 8u;
-        z1 = ZEROS ? v.ring[za + v.zero_rows] : 8u;
+        z1 = ZEROS ? v.ring[za + 8 * a.zero_bytes] : 8u;
+        if (second && 2 * pair + 1 >= v.blocks) s0 = s1 = 0.0f;   // what lies there is no scale
     }
 };
 
 // COUNT pairs of blocks from pair FIRST on, in one stretch without a branch, so that their loads, conversions and matrix
 // instructions overlap.  The products of a pair are summed by the matrix
 // instructions, one scale at a time (FINE: two scales in a pair).  Here in the type itself, for eight rows of x.
-template <typename H, bool FINE, bool ZEROS>
+template <typename H, bool FINE, bool ZEROS, int SPLIT>
 struct ByType {
+    static constexpr int kAtOnce = 1;
     template <int FIRST, int COUNT>
-    static __device__ __forceinline__ void multiply(float (&acc)[8], const uint32_t (&xr)[kMaxBlocks][4], const TileView& v) {
+    static __device__ __forceinline__ void multiply(float (&acc)[8], const uint32_t (&xr)[kMaxBlocks][4], const MatvecArgs& a, const TileView& v) {
         constexpr int kScales = FINE ? 2 : 1, kBlocks = 2 / kScales;   // scales of a pair, blocks of a scale
-        const Words<COUNT> w(v, FIRST);
+        const Words<SPLIT, COUNT> w(v, FIRST);
 #pragma unroll
         for (int p = 0; p < COUNT; ++p)
 #pragma unroll
             for (int i = 0; i < kScales; ++i) {
-                const Scales<H, ZEROS> s(v, FIRST + p, i != 0);
+                const Scales<H, ZEROS> s(a, v, FIRST + p, i != 0);
                 const uint32_t off0 = H::offset(s.z0), off1 = H::offset(s.z1);
                 float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
@@ -344,18 +347,19 @@ struct ByType {
 
 // By integers, for 2 * MMAS rows of x: column 4 r + d of a product is byte d of row r.  At most 64 products of 2^7 by 2^7 meet in
 // a sum, so it stays below 2^22 and kOne + sum is a float's bit pattern whose value is 1.5 * 2^23 + sum.
-template <typename H, bool FINE, bool ZEROS, int MMAS>
+template <typename H, bool FINE, bool ZEROS, int SPLIT, int MMAS>
 struct ByInteger {
+    static constexpr int kAtOnce = MMAS == 1 ? 2 : 1;
     static constexpr int kOne = 0x4b400000;
     template <int FIRST, int COUNT>
-    static __device__ __forceinline__ void multiply(float (&acc)[8], const uint32_t (&xr)[kMaxBlocks][4], const TileView& v) {
+    static __device__ __forceinline__ void multiply(float (&acc)[8], const uint32_t (&xr)[kMaxBlocks][4], const MatvecArgs& a, const TileView& v) {
         constexpr int kScales = FINE ? 2 : 1, kBlocks = 2 / kScales;
-        const Words<COUNT> w(v, FIRST);
+        const Words<SPLIT, COUNT> w(v, FIRST);
 #pragma unroll
         for (int p = 0; p < COUNT; ++p)
 #pragma unroll
             for (int i = 0; i < kScales; ++i) {
-                const Scales<H, ZEROS> s(v, FIRST + p, i != 0);
+                const Scales<H, ZEROS> s(a, v, FIRST + p, i != 0);
                 const uint32_t neg0 = (0u - s.z0 & 0xffu) * 0x01010101u, neg1 = (0u - s.z1 & 0xffu) * 0x01010101u;   // bytes -zero
                 int c[MMAS][4];
 #pragma unroll
@@ -386,18 +390,27 @@ struct ByInteger {
     }
 };
 
-// All of a warp's pairs, two at a time.
+// All of a warp's pairs, two at a time where the registers allow it.
 template <typename P, int FIRST = 0>
-__device__ __forceinline__ void multiply_pairs(float (&acc)[8], const uint32_t (&xr)[kMaxBlocks][4], const TileView& v, int pairs)
+__device__ __forceinline__ void multiply_pairs(float (&acc)[8], const uint32_t (&xr)[kMaxBlocks][4], const MatvecArgs& a, const TileView& v)
 {
     if constexpr (2 * FIRST < kMaxBlocks) {
-        if (pairs >= FIRST + 2) {
-            P::template multiply<FIRST, 2>(acc, xr, v);
-            multiply_pairs<P, FIRST + 2>(acc, xr, v, pairs);
-        } else if (pairs > FIRST) {
-            P::template multiply<FIRST, 1>(acc, xr, v);
+        if (v.blocks > 2 * (FIRST + P::kAtOnce - 1)) {
+            P::template multiply<FIRST, P::kAtOnce>(acc, xr, a, v);
+            multiply_pairs<P, FIRST + P::kAtOnce>(acc, xr, a, v);
+        } else if (v.blocks > 2 * FIRST) {
+            P::template multiply<FIRST, 1>(acc, xr, a, v);
         }
     }
+}
+
+// A tile's scales (or zero points) where they are no box: as they lie, in two halves if gated.
+__device__ __forceinline__ void copy_side(const MatvecArgs& a, const uint8_t* src, int bytes, int expert, int row, uint32_t to,
+                                          uint32_t bar) {
+    const int rows = a.gated ? kTileRows / 2 : kTileRows;
+    src += ((long long)expert * a.N + row) * bytes;
+    bulk_load(to, src, rows * bytes, bar);
+    if (a.gated) bulk_load(to + rows * bytes, src + (long long)(a.N / 2) * bytes, rows * bytes, bar);
 }
 
 // Row `i` of a run's x, from its member-th pair of blocks on.
@@ -409,18 +422,20 @@ __device__ __forceinline__ const uint8_t* x_row(const MatvecArgs& a, int row, in
 }
 
 // Block j of a warp exists, and its place behind the warp's first one (one that does not exist: the first one's).
+template <int SPLIT>
 __device__ __forceinline__ bool block_exists(const MatvecArgs& a, int member, int j) {
-    return (2 * (member + j / 2 * a.split) + j % 2) * 32 < a.K;
+    return (2 * (member + j / 2 * SPLIT) + j % 2) * 32 < a.K;
 }
+template <int SPLIT>
 __device__ __forceinline__ int x_block(const MatvecArgs& a, int member, int j) {
-    return block_exists(a, member, j) ? j / 2 * a.split * 128 + j % 2 * 64 : 0;
+    return block_exists<SPLIT>(a, member, j) ? j / 2 * SPLIT * 128 + j % 2 * 64 : 0;
 }
 
 // x for the products in its own type: thread (g, t) holds row g's columns 8t .. 8t+7 of each of its warp's blocks, as the pairs
 // (0, 4) (1, 5) (2, 6) (3, 7); zeros behind the last column.  A row of bf16 values near the end of fp32's range is held 2^16
-// times smaller, so that products with codes do not leave it; `unit` says so for rows 2t and 2t + 1.
-template <typename T>
-__device__ __forceinline__ void load_values(uint32_t (&xr)[kMaxBlocks][4], float (&unit)[2], const MatvecArgs& a, int row, int rows,
+// times smaller, so that products with codes do not leave it; `unit` says so.
+template <typename T, int SPLIT>
+__device__ __forceinline__ void load_values(uint32_t (&xr)[kMaxBlocks][4], float* unit, const MatvecArgs& a, int row, int rows,
                                             int member, int lane)
 {
     const int g = lane / 4, t = lane % 4;
@@ -429,27 +444,27 @@ __device__ __forceinline__ void load_values(uint32_t (&xr)[kMaxBlocks][4], float
         // without a branch, so that all are under way together
 #pragma unroll
         for (int j = 0; j < kMaxBlocks; ++j) {
-            const uint4 v = *reinterpret_cast<const uint4*>(xp + x_block(a, member, j));
+            const uint4 v = *reinterpret_cast<const uint4*>(xp + x_block<SPLIT>(a, member, j));
             xr[j][0] = v.x, xr[j][1] = v.y, xr[j][2] = v.z, xr[j][3] = v.w;
         }
     } else {
 #pragma unroll
         for (int j = 0; j < kMaxBlocks; ++j) {
-            const uint16_t* h = reinterpret_cast<const uint16_t*>(xp + x_block(a, member, j));
+            const uint16_t* h = reinterpret_cast<const uint16_t*>(xp + x_block<SPLIT>(a, member, j));
 #pragma unroll
             for (int i = 0; i < 4; ++i) xr[j][i] = (uint32_t)h[2 * i] | ((uint32_t)h[2 * i + 1] << 16);
         }
     }
 #pragma unroll
     for (int j = 0; j < kMaxBlocks; ++j) {
-        const bool there = block_exists(a, member, j);
+        const bool there = block_exists<SPLIT>(a, member, j);
         const uint32_t v0 = there ? xr[j][0] : 0, v1 = there ? xr[j][1] : 0, v2 = there ? xr[j][2] : 0, v3 = there ? xr[j][3] : 0;
         xr[j][0] = __byte_perm(v0, v2, 0x5410);
         xr[j][1] = __byte_perm(v0, v2, 0x7632);
         xr[j][2] = __byte_perm(v1, v3, 0x5410);
         xr[j][3] = __byte_perm(v1, v3, 0x7632);
     }
-    unit[0] = unit[1] = 1.0f;
+    float by_row = 1.0f;
     if constexpr (Half2<T>::kMantissa == 7) {
         uint32_t most = 0;
 #pragma unroll
@@ -465,20 +480,20 @@ __device__ __forceinline__ void load_values(uint32_t (&xr)[kMaxBlocks][4], float
             for (int j = 0; j < kMaxBlocks; ++j)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) asm("mul.rn.bf16x2 %0, %0, %1;" : "+r"(xr[j][i]) : "r"(by));
-            const unsigned rows_large = __ballot_sync(~0u, large);
-            if (rows_large >> (8 * t) & 1) unit[0] = 65536.0f;
-            if (rows_large >> (8 * t + 4) & 1) unit[1] = 65536.0f;
+            if (large) by_row = 65536.0f;
         }
     }
+    if (t == 0) unit[g] = by_row;
+    __syncwarp();
 }
 
 // x for the products by integers: thread (g, t) holds byte g % 4 of rows g / 4 and 2 + g / 4, of the columns 8t, 8t+2, 8t+4,
 // 8t+6 in one word and of the odd ones in the next.  A value is 31 bits below 2^e, the power of two above the largest of
 // its row's values in this warp, split into signed bytes.  Each thread converts two columns of a block; four threads'
-// words are then transposed byte by byte.  Returns the form that x is in (1 up to two rows, 2 up to four), or 0 if a value
-// is not finite.
-template <typename T>
-__device__ __forceinline__ int load_digits(uint32_t (&xr)[kMaxBlocks][4], float (&unit)[2], const MatvecArgs& a, int row, int rows,
+// words are then transposed byte by byte.  `unit` gets 2^(e - 1) of each row.  Returns the form that x is in (1 up to two rows, 2 up to four), or 0 if a value is not
+// finite.
+template <typename T, int SPLIT>
+__device__ __forceinline__ int load_digits(uint32_t (&xr)[kMaxBlocks][4], float* unit, const MatvecArgs& a, int row, int rows,
                                            int member, int lane)
 {
     const int t = lane % 4, q = lane / 4 % 4, forms = rows <= 2 ? 1 : 2;
@@ -490,17 +505,17 @@ __device__ __forceinline__ int load_digits(uint32_t (&xr)[kMaxBlocks][4], float 
         uint32_t raw[kMaxBlocks], most = 0;
         if (a.x_wide) {
 #pragma unroll
-            for (int j = 0; j < kMaxBlocks; ++j) raw[j] = *reinterpret_cast<const uint32_t*>(xp + x_block(a, member, j));
+            for (int j = 0; j < kMaxBlocks; ++j) raw[j] = *reinterpret_cast<const uint32_t*>(xp + x_block<SPLIT>(a, member, j));
         } else {
 #pragma unroll
             for (int j = 0; j < kMaxBlocks; ++j) {
-                const uint16_t* h = reinterpret_cast<const uint16_t*>(xp + x_block(a, member, j));
+                const uint16_t* h = reinterpret_cast<const uint16_t*>(xp + x_block<SPLIT>(a, member, j));
                 raw[j] = (uint32_t)h[0] | ((uint32_t)h[1] << 16);
             }
         }
 #pragma unroll
         for (int j = 0; j < kMaxBlocks; ++j) {
-            if (!block_exists(a, member, j)) raw[j] = 0;
+            if (!block_exists<SPLIT>(a, member, j)) raw[j] = 0;
             most = max(most, max(raw[j] & 0x7fffu, raw[j] >> 16 & 0x7fffu));
         }
 #pragma unroll
@@ -508,7 +523,7 @@ __device__ __forceinline__ int load_digits(uint32_t (&xr)[kMaxBlocks][4], float 
         if (__any_sync(~0u, most >= Half2<T>::kInf)) return 0;
         const int e = (int)(most >> Half2<T>::kMantissa) - Half2<T>::kBias + 1;   // all below 2^e
         const float scale = exp2_of(-e);
-        unit[m] = exp2_of(__shfl_sync(~0u, e, (t >> 1) * 16) - 1);
+        if (lane % 16 == 0) unit[2 * m + lane / 16] = exp2_of(e - 1);
 #pragma unroll
         for (int j = 0; j < kMaxBlocks; ++j)
 #pragma unroll
@@ -520,10 +535,11 @@ __device__ __forceinline__ int load_digits(uint32_t (&xr)[kMaxBlocks][4], float 
                 xr[j][2 * m + i] = v;
             }
     }
+    __syncwarp();
     return forms;
 }
 
-template <typename T, bool GATED, bool FINE, bool ZEROS>
+template <typename T, bool FINE, bool ZEROS, int SPLIT>
 __global__ void __launch_bounds__(kThreads, 1) matvec4_kernel(const MatvecArgs a, const __grid_constant__ MatvecMaps maps)
 {
     extern __shared__ uint8_t pool[];
@@ -613,60 +629,56 @@ __global__ void __launch_bounds__(kThreads, 1) matvec4_kernel(const MatvecArgs a
         __syncthreads();
     }
 
-    const int tiles = a.N / kTileRows, per_stage = kWarps / a.split, groups = a.K >> (5 + a.group_shift);
-    const unsigned begin = unit_at_share(ex, a, blockIdx.x, tiles), end = unit_at_share(ex, a, blockIdx.x + 1, tiles);
+    const int tiles = a.N / kTileRows;
+    constexpr int per_stage = kWarps / SPLIT;
+    if (threadIdx.x == 0) {
+        const unsigned begin = unit_at_share(ex, a, blockIdx.x, tiles), end = unit_at_share(ex, a, blockIdx.x + 1, tiles);
+        sh.begin = begin;
+        sh.end = end;
+        const int2 x = begin < end ? rows_of(ex, run_at(ex, a, begin, end, tiles)) : make_int2(-1, 0);
+        sh.start = {x.x, x.y, 0, 1};
+    }
+    __syncthreads();
     bool ok = true;
 
     if (warp >= kWarps) {
         setmaxnreg_dec<kOtherRegisters>();
         if (warp == kLoadWarp) {
-            // ---- the stages, one after the other, and the end
+            // ---- the stages, one after the other, and the end.  Lane m requests tile m of a stage.
             if (lane == 0) prefetch_tmap(&maps.codes);
-            const int rows = GATED ? kTileRows / 2 : kTileRows;
+            const int rows = a.gated ? kTileRows / 2 : kTileRows;
             int it = 0, slot = 0, lap = 0;
-            auto advance = [&] {
-                ++it;
-                if (++slot == a.stages) {
-                    slot = 0;
-                    lap ^= 1;
-                }
-            };
-            for (unsigned u = begin; u < end && ok;) {
-                const Run r = run_at(ex, a, u, end, tiles);
-                const int2 x = rows_of(ex, r);
+            for (unsigned u = sh.begin; u < sh.end && ok;) {
+                Run r = run_at(ex, a, u, sh.end, a.N / kTileRows);
                 u += r.count;
-                for (int t0 = 0; t0 < r.count; t0 += per_stage, advance()) {
+                for (; r.count > 0; r.count -= per_stage, r.tile += per_stage) {
                     ok = it < a.stages || mbar_wait(smem_u32(&sh.empty_bar[slot]), lap ^ 1, &sh.abort);
                     if (!__all_sync(~0u, ok)) { ok = false; break; }
-                    const int n = min(per_stage, r.count - t0);
-                    const uint32_t bar = smem_u32(&sh.full_bar[slot]), dst = ring0 + slot * a.stage_bytes;
+                    const int n = min(per_stage, r.count);
+                    const uint32_t bar = smem_u32(&sh.full_bar[slot]);
                     if (lane == 0) {
-                        sh.info[it % kStageInfos] = {x.x, x.y, r.tile + t0, n};
-                        const int scales = a.scale_box ? a.scale_bytes : groups * 2, zeros = a.zero_box ? a.zero_bytes : groups;
-                        mbar_expect_tx(bar, (uint32_t)(n * kTileRows) * (uint32_t)(a.chunks * 128 + scales + (ZEROS ? zeros : 0)));
+                        const int2 x = rows_of(ex, r);
+                        sh.info[it % kStageInfos] = {x.x, x.y, r.tile, n};
+                        mbar_expect_tx(bar, (uint32_t)n * a.tile_bytes);
                     }
                     __syncwarp();
-                    const int boxes = a.whole ? 1 : a.chunks;
-                    for (int i = lane; i < n * boxes; i += 32) {
-                        const int m = i / boxes, c = i - m * boxes;
-                        box_load_5d(dst + (m * a.chunks + c) * 2048, &maps.codes, bar, c * 128, (r.tile + t0 + m) * rows, 0, 0, r.expert);
-                    }
-                    // a tile's scales where they are no box: as they lie, in two halves if gated
-                    auto copy_side = [&](const uint8_t* src, int bytes, int tile, uint32_t to) {
-                        for (int half = 0; half < (GATED ? 2 : 1); ++half)
-                            bulk_load(to + half * rows * bytes, src + ((long long)r.expert * a.N + half * (a.N / 2) + tile * rows) * bytes,
-                                      rows * bytes, bar);
-                    };
-                    for (int m = lane; m < n; m += 32) {
-                        const int tile = r.tile + t0 + m;
-                        const uint32_t to = dst + a.scale_at + m * kTileRows * a.scale_bytes;
-                        if (a.scale_box) box_load_4d(to, &maps.scales, bar, 0, tile * rows, 0, r.expert);
-                        else copy_side(a.scales, groups * 2, tile, to);
+                    if (lane < n) {
+                        const int row = (r.tile + lane) * rows;
+                        uint32_t to = ring0 + slot * a.stage_bytes;
+                        for (int c = 0; c < (a.whole ? 1 : a.chunks); ++c)
+                            box_load_5d(to + (lane * a.chunks + c) * 2048, &maps.codes, bar, c * 128, row, 0, 0, r.expert);
+                        if (a.scale_box) box_load_4d(to + a.scale_at + lane * kTileRows * a.scale_bytes, &maps.scales, bar, 0, row, 0, r.expert);
+                        else copy_side(a, a.scales, a.scale_bytes, r.expert, row, to + a.scale_at + lane * kTileRows * a.scale_bytes, bar);
                         if (ZEROS) {
-                            const uint32_t zero_to = dst + a.zero_at + m * kTileRows * a.zero_bytes;
-                            if (a.zero_box) box_load_4d(zero_to, &maps.zeros, bar, 0, tile * rows, 0, r.expert);
-                            else copy_side(a.zeros, groups, tile, zero_to);
+                            to += a.zero_at + lane * kTileRows * a.zero_bytes;
+                            if (a.zero_box) box_load_4d(to, &maps.zeros, bar, 0, row, 0, r.expert);
+                            else copy_side(a, a.zeros, a.zero_bytes, r.expert, row, to, bar);
                         }
+                    }
+                    ++it;
+                    if (++slot == a.stages) {
+                        slot = 0;
+                        lap ^= 1;
                     }
                 }
             }
@@ -695,16 +707,17 @@ __global__ void __launch_bounds__(kThreads, 1) matvec4_kernel(const MatvecArgs a
                 const StageInfo s = sh.info[it % kStageInfos];
                 if (s.tiles == 0) break;
                 const float(*part)[128] = sh.part[b];
-                for (int v = warp - kLoadWarp - 1; v < s.tiles * (GATED ? 2 : 4); v += kSumWarps) {
-                    const int m = GATED ? v / 2 : v / 4, i = GATED ? v % 2 : v % 4, x_row = 2 * t + (i & 1);
+                for (int v = warp - kLoadWarp - 1; v < s.tiles * (a.gated ? 2 : 4); v += kSumWarps) {
+                    const int m = a.gated ? v / 2 : v / 4, i = a.gated ? v % 2 : v % 4, x_row = 2 * t + (i & 1);
                     float y = 0.0f, gate = 0.0f;
-                    for (int k = 0; k < a.split; ++k) {
-                        y += part[m * a.split + k][i * 32 + lane];
-                        if (GATED) gate += part[m * a.split + k][(i + 2) * 32 + lane];
+#pragma unroll 4
+                    for (int k = 0; k < SPLIT; ++k) {
+                        y += part[m * SPLIT + k][i * 32 + lane];
+                        if (a.gated) gate += part[m * SPLIT + k][(i + 2) * 32 + lane];
                     }
                     if (x_row < s.rows) {
-                        if (GATED) y = gate / (1.0f + __expf(-gate)) * y;
-                        const int col = GATED ? (s.tile + m) * 8 + g : (s.tile + m) * kTileRows + g + 8 * (i / 2);
+                        if (a.gated) y = gate / (1.0f + __expf(-gate)) * y;
+                        const int col = a.gated ? (s.tile + m) * 8 + g : (s.tile + m) * kTileRows + g + 8 * (i / 2);
                         reinterpret_cast<T*>(a.out + (s.row + x_row) * a.out_stride)[col] = H::round(y);
                     }
                 }
@@ -717,74 +730,52 @@ __global__ void __launch_bounds__(kThreads, 1) matvec4_kernel(const MatvecArgs a
 
     // ---- `split` warps share a tile's K range, tile m of the stage belongs to warps [m * split, (m + 1) * split)
     setmaxnreg_inc<kMultiplyRegisters>();
-    const int member = warp % a.split, of_stage = warp / a.split;
-    // every split-th pair of 32-column blocks; the last pair of an odd number of blocks has its second block's x zero
-    const int all_pairs = (a.K + 63) / 64, pairs = (all_pairs - member + a.split - 1) / a.split;
+    const int member = warp % SPLIT, of_stage = warp / SPLIT;
     const int g = lane / 4, t = lane % 4;
     TileView view;
     {
         const int unit = 2 * member % 8;   // 16-byte unit of the first pair's first block in its chunk
-        const int row = of_stage * kTileRows + g, group = member * 2 >> a.group_shift;
-        const int chunk = (of_stage * a.chunks + member / 4) * 2048 + g * 128 + 4 * t;
+        const int row = of_stage * kTileRows + g, group = member * 64 / a.group;
         view.ring = ring;
-        view.even = chunk + ((unit ^ g) << 4);
-        view.odd = chunk + (((unit + 1) ^ g) << 4);
+        view.even = (of_stage * a.chunks + member / 4) * 2048 + g * 128 + 4 * t + ((unit ^ g) << 4);
         view.scales = a.scale_at + row * a.scale_bytes + 2 * group;
         view.zeros = a.zero_at + row * a.zero_bytes + group;
-        view.scale_rows = 8 * a.scale_bytes;
-        view.zero_rows = 8 * a.zero_bytes;
-        view.pair_step = a.split * 512;
-        view.zero_step = a.split * 2 >> a.group_shift;
-        view.scale_step = 2 * view.zero_step;
-        view.last_scale = a.scale_at + row * a.scale_bytes + 2 * (groups - 1);
-        view.last_zero = a.zero_at + row * a.zero_bytes + groups - 1;
+        const int pairs = ((a.K + 63) / 64 - member + SPLIT - 1) / SPLIT;
+        view.blocks = pairs > 0 ? min(2 * pairs, a.K / 32 - 2 * (member + (pairs - 1) * SPLIT) + 2 * (pairs - 1)) : 0;
     }
     uint32_t xr[kMaxBlocks][4];
     int form = 0;                      // 0 in the type itself, 1 by integers for up to two rows, 2 for up to four
-    // by integers, half of the power of two above the largest value of rows t / 2 and 2 + t / 2 of x; else see load_values
-    float unit[2] = {0.0f, 0.0f};
+    float* const unit = sh.unit[warp];
     int slot = 0, lap = 0, row = -1;
-    int2 next = {-1, 0};               // rows of x to take up: at first those of the first run, while its weights are on their way
-    if (begin < end) next = rows_of(ex, run_at(ex, a, begin, end, tiles));
-    StageInfo s = {};
-    bool arrived = false;
-    for (int it = 0;;) {
-        if (next.x != row) {
-            row = next.x;
-            form = 0;
-            if (next.y <= kFewRows) form = load_digits<T>(xr, unit, a, row, next.y, member, lane);
-            if (form == 0) load_values<T>(xr, unit, a, row, next.y, member, lane);
-        }
-        const int b = it & 1;
-        if (!arrived) {
+    // round -1 only takes up the first x, while its weights are on their way
+    for (int it = -1;; ++it) {
+        if (it >= 0) {
             ok = mbar_wait(smem_u32(&sh.full_bar[slot]), lap, &sh.abort);
             if (!ok) break;
-            s = sh.info[it % kStageInfos];
-            if (s.tiles == 0) {
-                // the adding warps see the end, too; not before all have arrived for the stage two before it
-                if (it >= 2) ok = mbar_wait(smem_u32(&sh.free_bar[b]), (it >> 1) - 1 & 1, &sh.abort);
-                if (ok && lane == 0) mbar_arrive(smem_u32(&sh.done_bar[b]));
-                break;
-            }
-            arrived = true;
-            if (s.row != row) {
-                next = {s.row, s.rows};
-                continue;
-            }
         }
+        const StageInfo& s = it < 0 ? sh.start : sh.info[it % kStageInfos];
+        const int b = it & 1;
+        if (s.tiles == 0) {
+            // the adding warps see the end, too; not before all have arrived for the stage two before it
+            if (it >= 2) ok = mbar_wait(smem_u32(&sh.free_bar[b]), (it >> 1) - 1 & 1, &sh.abort);
+            if (ok && lane == 0) mbar_arrive(smem_u32(&sh.done_bar[b]));
+            break;
+        }
+        if (s.row != row) {
+            row = s.row;
+            form = 0;
+            if (s.rows <= kFewRows) form = load_digits<T, SPLIT>(xr, unit, a, row, s.rows, member, lane);
+            if (form == 0) load_values<T, SPLIT>(xr, unit, a, row, s.rows, member, lane);
+        }
+        if (it < 0) continue;
         float acc[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
         if (of_stage < s.tiles) {
             TileView v = view;
             const int at = slot * a.stage_bytes;
-            v.even += at;
-            v.odd += at;
-            v.scales += at;
-            v.zeros += at;
-            v.last_scale += at;
-            v.last_zero += at;
-            if (form == 1) multiply_pairs<ByInteger<H, FINE, ZEROS, 1>>(acc, xr, v, pairs);
-            else if (form == 2) multiply_pairs<ByInteger<H, FINE, ZEROS, 2>>(acc, xr, v, pairs);
-            else multiply_pairs<ByType<H, FINE, ZEROS>>(acc, xr, v, pairs);
+            v.ring += at;
+            if (form == 1) multiply_pairs<ByInteger<H, FINE, ZEROS, SPLIT, 1>>(acc, xr, a, v);
+            else if (form == 2) multiply_pairs<ByInteger<H, FINE, ZEROS, SPLIT, 2>>(acc, xr, a, v);
+            else multiply_pairs<ByType<H, FINE, ZEROS, SPLIT>>(acc, xr, a, v);
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(smem_u32(&sh.empty_bar[slot]));
@@ -793,15 +784,15 @@ __global__ void __launch_bounds__(kThreads, 1) matvec4_kernel(const MatvecArgs a
         float* part = sh.part[b][warp];
         if (form == 0) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) part[i * 32 + lane] = acc[i] * unit[i & 1];
+            for (int i = 0; i < 4; ++i) part[i * 32 + lane] = acc[i] * unit[2 * t + (i & 1)];
         } else {
             // this thread's columns 2t, 2t + 1 are bytes 0, 1 (t even) or 2, 3 of x row t / 2 (and 2 + t / 2)
             const float low = (t & 1 ? 65536.0f : 1.0f) * (ZEROS ? 0x1p-29f : 0x1p-33f);
 #pragma unroll
             for (int m = 0; m < 2; ++m) {
                 if (m >= form) break;
-                float y0 = fmaf(256.0f, acc[4 * m + 1], acc[4 * m]) * low * unit[m];
-                float y1 = fmaf(256.0f, acc[4 * m + 3], acc[4 * m + 2]) * low * unit[m];
+                float y0 = fmaf(256.0f, acc[4 * m + 1], acc[4 * m]) * low * unit[2 * m + (t >> 1)];
+                float y1 = fmaf(256.0f, acc[4 * m + 3], acc[4 * m + 2]) * low * unit[2 * m + (t >> 1)];
                 y0 += __shfl_xor_sync(~0u, y0, 1);
                 y1 += __shfl_xor_sync(~0u, y1, 1);
                 part[((t & 1) * 2 + (t >> 1)) * 32 + g * 4 + m] = t & 1 ? y1 : y0;
@@ -813,15 +804,13 @@ __global__ void __launch_bounds__(kThreads, 1) matvec4_kernel(const MatvecArgs a
             slot = 0;
             lap ^= 1;
         }
-        ++it;
-        arrived = false;
     }
     if (!ok) {
         // a load that never came, or sums that nobody added: the results are NaN
-        for (unsigned u = begin + warp; u < end; u += kWarps) {
-            const Run r = run_at(ex, a, u, u + 1, tiles);
+        for (unsigned u = sh.begin + warp; u < sh.end; u += kWarps) {
+            const Run r = run_at(ex, a, u, u + 1, a.N / kTileRows);
             const int2 x = rows_of(ex, r);
-            const int cols = GATED ? 8 : kTileRows;
+            const int cols = a.gated ? kTileRows / 2 : kTileRows;
             for (int i = lane; i < x.y * cols; i += 32)
                 reinterpret_cast<T*>(a.out + (x.x + i / cols) * a.out_stride)[r.tile * cols + i % cols] = H::round(__int_as_float(0x7fc00000));
         }
@@ -835,29 +824,30 @@ using namespace moe;
 
 namespace {
 
-template <typename T, bool GATED, bool FINE, bool ZEROS>
+template <typename T, bool FINE, bool ZEROS, int SPLIT>
 cudaError_t launch_form(const MatvecArgs& a, const MatvecMaps& maps, int sms, cudaStream_t stream)
 {
     const size_t smem = (size_t)a.stages * a.stage_bytes + experts_bytes(a.E) + kSwizzleAtom;
-    const auto kernel = matvec4_kernel<T, GATED, FINE, ZEROS>;
+    const auto kernel = matvec4_kernel<T, FINE, ZEROS, SPLIT>;
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return e;
     return launch_after(kernel, dim3(sms), dim3(kThreads), smem, 1, stream, a, maps);
 }
 
-template <typename T, bool GATED>
-cudaError_t launch_groups(const MatvecArgs& a, const MatvecMaps& maps, int sms, cudaStream_t stream)
+template <typename T, bool FINE, bool ZEROS>
+cudaError_t launch_split(const MatvecArgs& a, const MatvecMaps& maps, int split, int sms, cudaStream_t stream)
 {
-    const bool zeros = a.zeros != nullptr;
-    if (a.group_shift == 0)
-        return zeros ? launch_form<T, GATED, true, true>(a, maps, sms, stream) : launch_form<T, GATED, true, false>(a, maps, sms, stream);
-    return zeros ? launch_form<T, GATED, false, true>(a, maps, sms, stream) : launch_form<T, GATED, false, false>(a, maps, sms, stream);
+    return split == 4   ? launch_form<T, FINE, ZEROS, 4>(a, maps, sms, stream)
+           : split == 8 ? launch_form<T, FINE, ZEROS, 8>(a, maps, sms, stream)
+                        : launch_form<T, FINE, ZEROS, 16>(a, maps, sms, stream);
 }
 
 template <typename T>
-cudaError_t launch_matvec(const MatvecArgs& a, const MatvecMaps& maps, bool gated, int sms, cudaStream_t stream)
+cudaError_t launch_matvec(const MatvecArgs& a, const MatvecMaps& maps, int split, int sms, cudaStream_t stream)
 {
-    return gated ? launch_groups<T, true>(a, maps, sms, stream) : launch_groups<T, false>(a, maps, sms, stream);
+    if (a.group == 32)
+        return a.zeros ? launch_split<T, true, true>(a, maps, split, sms, stream) : launch_split<T, true, false>(a, maps, split, sms, stream);
+    return a.zeros ? launch_split<T, false, true>(a, maps, split, sms, stream) : launch_split<T, false, false>(a, maps, split, sms, stream);
 }
 
 // A weight tensor [E, n, row_bytes] as boxes of a tile's sixteen rows (gated: eight of each half) and `box_bytes` of each;
@@ -946,7 +936,8 @@ extern "C" int moe_fp8_b200_matvec_w4(const void* x, int64_t x_stride, int by_to
     a.E = w->num_experts;
     a.N = w->n;
     a.K = w->k;
-    a.group_shift = w->group == 32 ? 0 : w->group == 64 ? 1 : 2;
+    a.group = w->group;
+    a.gated = gated ? 1 : 0;
     a.rows = (int)rows;
     a.share_step = (unsigned)(((uint64_t)1 << 32) / (unsigned)sms);
     a.prefetch = x_rows * w->k * 2 <= ((int64_t)4 << 20);
@@ -957,13 +948,14 @@ extern "C" int moe_fp8_b200_matvec_w4(const void* x, int64_t x_stride, int by_to
         a.row_pair = plan->row_pair;
     }
     // a warp holds at most kMaxBlocks blocks of x
-    a.split = w->k <= 32 * kMaxBlocks * 4 ? 4 : w->k <= 32 * kMaxBlocks * 8 ? 8 : 16;
+    const int split = w->k <= 32 * kMaxBlocks * 4 ? 4 : w->k <= 32 * kMaxBlocks * 8 ? 8 : 16;
     a.chunks = (w->k / 2 + 127) / 128;
     a.whole = w->k % 256 == 0;
     // Scales and zero points come as boxes a little wider than their rows: eight rows start in different groups of four banks
     // if their pitch is an odd number of 16-byte units (a box has at most 256 values; K = 8192 with groups of 32 has that many)
     auto pitch = [](int bytes, int most) { return bytes % 32 || bytes >= most ? bytes : bytes + 16; };
-    const int per_stage = kWarps / a.split;
+    const int per_stage = kWarps / split;
+    a.scale_step = 64 * split / w->group;
     a.scale_box = groups * 2 % 16 == 0;
     a.zero_box = groups % 16 == 0;
     a.scale_bytes = a.scale_box ? pitch(groups * 2, 512) : groups * 2;
@@ -973,13 +965,13 @@ extern "C" int moe_fp8_b200_matvec_w4(const void* x, int64_t x_stride, int by_to
     a.stage_bytes = (a.zero_at + (w->zeros ? per_stage * kTileRows * a.zero_bytes : 0) + 1023) / 1024 * 1024;
     a.stages = (int)((kSharedLimit - sizeof(Shared) - experts_bytes(a.E) - kSwizzleAtom - 256) / a.stage_bytes);
     if (a.stages > kMaxStages) a.stages = kMaxStages;
+    a.tile_bytes = kTileRows * (unsigned)(a.chunks * 128 + a.scale_bytes + (w->zeros ? a.zero_bytes : 0));
     MatvecMaps maps = {};
     int r = encode_weights(maps.codes, w->codes, a, gated != 0, w->k / 2, 128, true);
     if (r == 0 && a.scale_box) r = encode_weights(maps.scales, w->scales, a, gated != 0, groups * 2, a.scale_bytes, false);
     if (r == 0 && w->zeros && a.zero_box) r = encode_weights(maps.zeros, w->zeros, a, gated != 0, groups, a.zero_bytes, false);
     if (r != 0) return refuse(err, err_len, MOE_FP8_B200_ERR_CUDA, "cuTensorMapEncodeTiled(weights) failed: %d", r);
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
-    e = dtype == MOE_FP8_B200_BF16 ? launch_matvec<__nv_bfloat16>(a, maps, gated != 0, sms, s)
-                                    : launch_matvec<__half>(a, maps, gated != 0, sms, s);
+    e = dtype == MOE_FP8_B200_BF16 ? launch_matvec<__nv_bfloat16>(a, maps, split, sms, s) : launch_matvec<__half>(a, maps, split, sms, s);
     return e == cudaSuccess ? MOE_FP8_B200_OK : refuse(err, err_len, MOE_FP8_B200_ERR_CUDA, "launch failed: %s", cudaGetErrorString(e));
 }
