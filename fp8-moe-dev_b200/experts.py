@@ -14,6 +14,7 @@ inside the reference's layer are kernel/moe_fp8.cu:1064-1115 (permute) and :2254
 from __future__ import annotations
 
 import ctypes as C
+import threading
 from typing import Optional, Tuple
 
 import torch
@@ -24,58 +25,70 @@ from .op import MoeError
 _ROW_TYPES = {torch.bfloat16: _lib.BF16, torch.float16: _lib.FP16, torch.float32: _lib.FP32}
 _ID_BITS = {torch.int32: 32, torch.int64: 64}
 _raw_stream = torch._C._cuda_getCurrentRawStream
-_ERR_BYTES = 256
+_current_device = torch._C._cuda_getDevice
 _SMALL = 1 << 20   # tokens up to which a plan's size needs no word from the library
 
 
-def _call(fn, device, *args):
-    """fn(*args, stream, err, err_len) with the tensors' device current."""
-    err = C.create_string_buffer(_ERR_BYTES)
-    index = device.index
-    if index == torch.cuda.current_device():
-        rc = fn(*args, _raw_stream(index), err, _ERR_BYTES)
+class _Text(threading.local):
+    """A thread's buffer for error messages."""
+
+    def __init__(self):
+        self.buffer = C.create_string_buffer(256)
+
+
+_text = _Text()
+
+
+def _call(fn, index, *args):
+    """fn(*args, stream, err, err_len) with GPU `index` current."""
+    err = _text.buffer
+    if index == _current_device():
+        rc = fn(*args, _raw_stream(index), err, 256)
     else:
         with torch.cuda.device(index):
-            rc = fn(*args, _raw_stream(index), err, _ERR_BYTES)
+            rc = fn(*args, _raw_stream(index), err, 256)
     if rc != _lib.OK:
         raise MoeError(rc, err.value.decode())
 
 
+# The checks are written out and compare GPU indices, not device objects: small calls are bound by the host's time.
 def _on_gpu(name, t):
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a torch.Tensor")
-    if not t.is_cuda:
+    index = t.get_device()
+    if index < 0 or not t.is_cuda:
         raise ValueError(f"{name} must live on a CUDA device, got {t.device}")
-    return t.device
+    return index
 
 
-def _packed(name, t, dtype, shape, device):
+def _wrong(name, t, dtype, shape, index):
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a torch.Tensor")
     if t.dtype != dtype:
         raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
-    if t.shape != shape:
+    if tuple(t.shape) != tuple(shape):
         raise ValueError(f"{name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
-    if not t.is_contiguous():
-        raise ValueError(f"{name} must be contiguous")
-    if t.device != device:
-        raise ValueError(f"{name} must live on {device}, got {t.device}")
+    if not t.is_cuda or t.get_device() != index:
+        raise ValueError(f"{name} must live on cuda:{index}, got {t.device}")
+    raise ValueError(f"{name} must be contiguous")
+
+
+def _packed(name, t, dtype, shape, index):
+    """The address of a contiguous tensor."""
+    if (not isinstance(t, torch.Tensor) or t.dtype is not dtype or t.shape != shape or not t.is_contiguous() or not t.is_cuda
+            or t.get_device() != index):
+        _wrong(name, t, dtype, shape, index)
     return t.data_ptr()
 
 
-def _matrix(name, t, rows, columns, dtype, device):
+def _matrix(name, t, rows, columns, dtype, index):
     """A [rows, columns] matrix whose rows are contiguous, at any stride: its address and stride."""
-    if not isinstance(t, torch.Tensor):
-        raise TypeError(f"{name} must be a torch.Tensor")
-    if t.dtype != dtype:
-        raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
-    if t.dim() != 2 or t.shape[0] != rows or t.shape[1] != columns:
-        raise ValueError(f"{name} must have shape ({rows}, {columns}), got {tuple(t.shape)}")
+    if (not isinstance(t, torch.Tensor) or t.dtype is not dtype or t.shape != (rows, columns) or not t.is_cuda
+            or t.get_device() != index):
+        _wrong(name, t, dtype, (rows, columns), index)
     stride, column = t.stride()
     if column != 1 and columns > 1:
         raise ValueError(f"{name}: the elements of a row must be contiguous")
-    if t.device != device:
-        raise ValueError(f"{name} must live on {device}, got {t.device}")
     return t.data_ptr(), stride
 
 
@@ -111,22 +124,23 @@ class ExpertPlan:
 
     Made by sort_tokens, or from four tensors of one's own (to be filled, or filled elsewhere)."""
     __slots__ = ("pair_row", "row_pair", "expert_offset", "expert_count", "align", "num_tokens", "top_k", "num_experts",
-                 "capacity", "device", "_c")
+                 "capacity", "device", "index", "_c")
 
     def __init__(self, pair_row, row_pair, expert_offset, expert_count, *, align: int = 1):
-        device = _on_gpu("pair_row", pair_row)
+        index = _on_gpu("pair_row", pair_row)
         if pair_row.dim() != 2:
             raise ValueError(f"pair_row must have shape (tokens, top_k), got {tuple(pair_row.shape)}")
         T, K = pair_row.shape
         E = expert_count.shape[0] if isinstance(expert_count, torch.Tensor) and expert_count.dim() == 1 else 0
-        self.num_tokens, self.top_k, self.num_experts, self.align = T, K, E, int(align)
-        self.capacity = plan_rows(T, K, E, self.align)
+        self.num_tokens, self.top_k, self.num_experts, self.align = T, K, E, align
+        self.capacity = capacity = plan_rows(T, K, E, align)
         self.pair_row, self.row_pair, self.expert_offset, self.expert_count = pair_row, row_pair, expert_offset, expert_count
-        self.device = device
-        self._c = C.byref(_lib.Plan(T, K, E, self.align, _packed("pair_row", pair_row, torch.int32, (T, K), device),
-                                    _packed("row_pair", row_pair, torch.int32, (self.capacity,), device),
-                                    _packed("expert_offset", expert_offset, torch.int32, (E + 1,), device),
-                                    _packed("expert_count", expert_count, torch.int32, (E,), device)))
+        self.device, self.index = pair_row.device, index
+        i32 = torch.int32
+        self._c = C.byref(_lib.Plan(T, K, E, align, _packed("pair_row", pair_row, i32, (T, K), index),
+                                    _packed("row_pair", row_pair, i32, (capacity,), index),
+                                    _packed("expert_offset", expert_offset, i32, (E + 1,), index),
+                                    _packed("expert_count", expert_count, i32, (E,), index)))
 
     @classmethod
     def empty(cls, num_tokens: int, top_k: int, num_experts: int, align: int = 1, device="cuda") -> "ExpertPlan":
@@ -140,12 +154,12 @@ class ExpertPlan:
 def _check_plan(plan):
     if not isinstance(plan, ExpertPlan):
         raise TypeError("plan must be an ExpertPlan")
-    return plan.device
+    return plan.index
 
 
 def _ids(topk_idx, num_experts, align, plan):
     """The plan to fill for these ids."""
-    device = _on_gpu("topk_idx", topk_idx)
+    index = _on_gpu("topk_idx", topk_idx)
     if topk_idx.dtype not in _ID_BITS:
         raise TypeError(f"topk_idx must be int32 or int64, got {topk_idx.dtype}")
     if topk_idx.dim() != 2:
@@ -154,9 +168,9 @@ def _ids(topk_idx, num_experts, align, plan):
         raise ValueError("topk_idx must be contiguous")
     T, K = topk_idx.shape
     if plan is None:
-        return ExpertPlan.empty(T, K, int(num_experts), int(align), device)
-    if _check_plan(plan) != device:
-        raise ValueError(f"plan must live on {device}, got {plan.device}")
+        return ExpertPlan.empty(T, K, int(num_experts), int(align), topk_idx.device)
+    if _check_plan(plan) != index:
+        raise ValueError(f"plan must live on {topk_idx.device}, got {plan.device}")
     if (plan.num_tokens, plan.top_k, plan.num_experts, plan.align) != (T, K, num_experts, align):
         raise ValueError(f"plan is for {plan.num_tokens} tokens, top_k {plan.top_k}, {plan.num_experts} experts, align {plan.align}; "
                          f"the call has {T}, {K}, {num_experts}, {align}")
@@ -168,7 +182,7 @@ def sort_tokens(topk_idx, num_experts: int, *, first_expert: int = 0, align: int
     """Sorts the (token, expert) pairs of topk_idx [T, top_k] (int32 or int64) by expert.  The plan's experts are
     [first_expert, first_expert + num_experts); pairs of other experts (an id of -1, another GPU's expert) have no row."""
     plan = _ids(topk_idx, num_experts, align, plan)
-    _call(_lib.load().moe_fp8_b200_sort_tokens, plan.device, topk_idx.data_ptr(), _ID_BITS[topk_idx.dtype], first_expert,
+    _call(_lib.load().moe_fp8_b200_sort_tokens, plan.index, topk_idx.data_ptr(), _ID_BITS[topk_idx.dtype], first_expert,
           plan._c)
     return plan
 
@@ -177,16 +191,16 @@ def _rows_for(x, plan, rows):
     """Arguments of the copy to packed rows: the matrix, and its C arguments."""
     kind = _row_type("x", x)
     H = x.shape[1]
-    xp, xs = _matrix("x", x, plan.num_tokens, H, x.dtype, plan.device)
+    xp, xs = _matrix("x", x, plan.num_tokens, H, x.dtype, plan.index)
     fresh = rows is None
     if fresh:
         rows = torch.empty((plan.capacity, H), dtype=x.dtype, device=plan.device)
-    rp, rs = _matrix("rows", rows, plan.capacity, H, x.dtype, plan.device)
+    rp, rs = _matrix("rows", rows, plan.capacity, H, x.dtype, plan.index)
     return rows, (xp, xs, rp, rs, kind, H, plan._c, int(fresh))
 
 
-def _wants_grad(*tensors):
-    return torch.is_grad_enabled() and any(t.requires_grad for t in tensors)
+def _wants_grad(a, b=None):
+    return (a.requires_grad or (b is not None and b.requires_grad)) and torch.is_grad_enabled()
 
 
 def dispatch(x, plan: ExpertPlan, rows=None):
@@ -199,7 +213,7 @@ def dispatch(x, plan: ExpertPlan, rows=None):
             raise ValueError("rows cannot be given where x requires a gradient")
         return _Dispatch.apply(x, plan)
     rows, args = _rows_for(x, plan, rows)
-    _call(_lib.load().moe_fp8_b200_dispatch_rows, plan.device, *args)
+    _call(_lib.load().moe_fp8_b200_dispatch_rows, plan.index, *args)
     return rows
 
 
@@ -210,7 +224,7 @@ def sort_and_dispatch(x, topk_idx, num_experts: int, *, first_expert: int = 0, a
     if _wants_grad(x):
         return dispatch(x, sort_tokens(topk_idx, num_experts, first_expert=first_expert, align=align, plan=plan), rows), plan
     rows, args = _rows_for(x, plan, rows)
-    _call(_lib.load().moe_fp8_b200_sort_and_dispatch, plan.device, topk_idx.data_ptr(), _ID_BITS[topk_idx.dtype], first_expert,
+    _call(_lib.load().moe_fp8_b200_sort_and_dispatch, plan.index, topk_idx.data_ptr(), _ID_BITS[topk_idx.dtype], first_expert,
           *args)
     return rows, plan
 
@@ -218,12 +232,12 @@ def sort_and_dispatch(x, topk_idx, num_experts: int, *, first_expert: int = 0, a
 def _combine(y, weights, plan, out):
     kind = _row_type("y", y)
     H = y.shape[1]
-    yp, ys = _matrix("y", y, plan.capacity, H, y.dtype, plan.device)
-    wp = None if weights is None else _packed("weights", weights, torch.float32, (plan.num_tokens, plan.top_k), plan.device)
+    yp, ys = _matrix("y", y, plan.capacity, H, y.dtype, plan.index)
+    wp = None if weights is None else _packed("weights", weights, torch.float32, (plan.num_tokens, plan.top_k), plan.index)
     if out is None:
         out = torch.empty((plan.num_tokens, H), dtype=y.dtype, device=plan.device)
-    op, os = _matrix("out", out, plan.num_tokens, H, y.dtype, plan.device)
-    _call(_lib.load().moe_fp8_b200_combine_rows, plan.device, yp, ys, wp, op, os, kind, H, plan._c)
+    op, os = _matrix("out", out, plan.num_tokens, H, y.dtype, plan.index)
+    _call(_lib.load().moe_fp8_b200_combine_rows, plan.index, yp, ys, wp, op, os, kind, H, plan._c)
     return out
 
 
@@ -252,21 +266,21 @@ def combine_backward(grad_out, y, weights, plan: ExpertPlan, grad_y=None, grad_w
     not needed is None."""
     _check_plan(plan)
     kind = _row_type("grad_out", grad_out)
-    H, dtype, device = grad_out.shape[1], grad_out.dtype, plan.device
-    gp, gs = _matrix("grad_out", grad_out, plan.num_tokens, H, dtype, device)
-    yp, ys = _matrix("y", y, plan.capacity, H, dtype, device)
-    wp = _packed("weights", weights, torch.float32, (plan.num_tokens, plan.top_k), device)
+    H, dtype, device, index = grad_out.shape[1], grad_out.dtype, plan.device, plan.index
+    gp, gs = _matrix("grad_out", grad_out, plan.num_tokens, H, dtype, index)
+    yp, ys = _matrix("y", y, plan.capacity, H, dtype, index)
+    wp = _packed("weights", weights, torch.float32, (plan.num_tokens, plan.top_k), index)
     dp, ds, dwp = None, 0, None
     fresh = grad_y is None
     if need_y:
         if fresh:
             grad_y = torch.empty((plan.capacity, H), dtype=dtype, device=device)
-        dp, ds = _matrix("grad_y", grad_y, plan.capacity, H, dtype, device)
+        dp, ds = _matrix("grad_y", grad_y, plan.capacity, H, dtype, index)
     if need_weights:
         if grad_weights is None:
             grad_weights = torch.empty((plan.num_tokens, plan.top_k), dtype=torch.float32, device=device)
-        dwp = _packed("grad_weights", grad_weights, torch.float32, (plan.num_tokens, plan.top_k), device)
-    _call(_lib.load().moe_fp8_b200_combine_rows_backward, device, gp, gs, yp, ys, wp, dp, ds, dwp, kind, H, plan._c,
+        dwp = _packed("grad_weights", grad_weights, torch.float32, (plan.num_tokens, plan.top_k), index)
+    _call(_lib.load().moe_fp8_b200_combine_rows_backward, index, gp, gs, yp, ys, wp, dp, ds, dwp, kind, H, plan._c,
           int(fresh))
     return grad_y if need_y else None, grad_weights if need_weights else None
 
@@ -286,14 +300,14 @@ def matvec_w4(x, codes, scales, *, zeros=None, plan: Optional[ExpertPlan] = None
     gated: the weights hold n / 2 linear rows, then n / 2 gated ones, and out [.., n / 2] is silu(gated) * linear.
     x is bfloat16 or float16; n a multiple of 16, k of the group and at most 8192.  The weights are read once per eight
     rows of an expert: for decode batches."""
-    device = _on_gpu("x", x)
+    index = _on_gpu("x", x)
     kind = _row_type("x", x)
     if kind == _lib.FP32:
         raise TypeError("x must be bfloat16 or float16, got torch.float32")
     if _wants_grad(x) or (isinstance(scales, torch.Tensor) and _wants_grad(scales)):
         raise ValueError("matvec_w4 has no gradient: call it under torch.no_grad()")
-    if plan is not None and _check_plan(plan) != device:
-        raise ValueError(f"plan must live on {device}, got {plan.device}")
+    if plan is not None and _check_plan(plan) != index:
+        raise ValueError(f"plan must live on {x.device}, got {plan.device}")
     if by_token and plan is None:
         raise ValueError("by_token needs a plan")
     K = x.shape[1]
@@ -306,16 +320,16 @@ def matvec_w4(x, codes, scales, *, zeros=None, plan: Optional[ExpertPlan] = None
     N, G = codes.shape[-2], scales.shape[-1]
     if G < 1 or K % G or K % 2:
         raise ValueError(f"scales of {G} groups do not divide {K} columns")
-    cp = _packed("codes", codes, torch.uint8, (*lead, N, K // 2), device)
-    sp = _packed("scales", scales, x.dtype, (*lead, N, G), device)
-    zp = None if zeros is None else _packed("zeros", zeros, torch.uint8, (*lead, N, G), device)
+    cp = _packed("codes", codes, torch.uint8, (*lead, N, K // 2), index)
+    sp = _packed("scales", scales, x.dtype, (*lead, N, G), index)
+    zp = None if zeros is None else _packed("zeros", zeros, torch.uint8, (*lead, N, G), index)
     rows = x.shape[0] if plan is None else plan.capacity
-    xp, xs = _matrix("x", x, plan.num_tokens if by_token else rows, K, x.dtype, device)
+    xp, xs = _matrix("x", x, plan.num_tokens if by_token else rows, K, x.dtype, index)
     columns = N // 2 if gated else N
     if out is None:
-        out = torch.empty((rows, columns), dtype=x.dtype, device=device)
-    op, os = _matrix("out", out, rows, columns, x.dtype, device)
-    _call(_lib.load().moe_fp8_b200_matvec_w4, device, xp, xs, int(by_token), C.byref(_lib.W4(cp, sp, zp, E, N, K, K // G)),
+        out = torch.empty((rows, columns), dtype=x.dtype, device=x.device)
+    op, os = _matrix("out", out, rows, columns, x.dtype, index)
+    _call(_lib.load().moe_fp8_b200_matvec_w4, index, xp, xs, int(by_token), C.byref(_lib.W4(cp, sp, zp, E, N, K, K // G)),
           int(gated), op, os, kind, None if plan is None else plan._c, rows)
     return out
 
