@@ -8,6 +8,7 @@
 #include <cuda_runtime.h>
 
 #include <cstring>
+#include <initializer_list>
 #include <type_traits>
 
 #include "call_checks.cuh"
@@ -234,7 +235,7 @@ __global__ void __launch_bounds__(kSortThreads) sort_tokens_kernel(const Id* ids
 }
 
 // ---------------------------------------------------------------------------------------
-// Row types: a piece of N elements, 16 bytes where the rows allow it, else one element.
+// Row types: a piece of N elements, 16 bytes where the rows allow it, else 8, 4 or 2.
 // ---------------------------------------------------------------------------------------
 // A piece stays in 32-bit words until its elements are used: as elements, eight bf16 values take eight registers (the
 // combine kernel 100 instead of 64, at half the loads in flight).
@@ -242,8 +243,9 @@ template <typename T, int N>
 struct Piece {
     typedef T Type;
     static constexpr int kBytes = sizeof(T) * N;
-    static_assert(kBytes == 16 || N == 1, "16 bytes, or one element");
-    typedef typename std::conditional<kBytes == 16, uint4, typename std::conditional<kBytes == 4, uint32_t, uint16_t>::type>::type Raw;
+    static_assert(kBytes == 16 || kBytes == 8 || kBytes == 4 || kBytes == 2, "one load");
+    typedef typename std::conditional<kBytes >= 8, typename std::conditional<kBytes == 16, uint4, uint2>::type,
+                                      typename std::conditional<kBytes == 4, uint32_t, uint16_t>::type>::type Raw;
     Raw raw;
     __device__ __forceinline__ uint32_t& word(int i) { return reinterpret_cast<uint32_t*>(&raw)[i]; }
     __device__ __forceinline__ uint32_t word(int i) const { return reinterpret_cast<const uint32_t*>(&raw)[i]; }
@@ -265,10 +267,8 @@ __device__ __forceinline__ uint32_t pack_halves(float lo, float hi, __half) {
 template <typename T, int N>
 __device__ __forceinline__ void unpack(const Piece<T, N>& p, float (&f)[N]) {
     if constexpr (sizeof(T) == 4) {
-        if constexpr (N == 1) f[0] = __uint_as_float(p.raw);
-        else
 #pragma unroll
-            for (int i = 0; i < N; ++i) f[i] = __uint_as_float(p.word(i));
+        for (int i = 0; i < N; ++i) f[i] = __uint_as_float(p.word(i));
     } else if constexpr (N == 1) {
         f[0] = low_half(p.raw, T{});
     } else {
@@ -282,10 +282,8 @@ __device__ __forceinline__ void unpack(const Piece<T, N>& p, float (&f)[N]) {
 template <typename T, int N>
 __device__ __forceinline__ void pack(const float (&f)[N], Piece<T, N>& p) {
     if constexpr (sizeof(T) == 4) {
-        if constexpr (N == 1) p.raw = __float_as_uint(f[0]);
-        else
 #pragma unroll
-            for (int i = 0; i < N; ++i) p.word(i) = __float_as_uint(f[i]);
+        for (int i = 0; i < N; ++i) p.word(i) = __float_as_uint(f[i]);
     } else if constexpr (N == 1) {
         p.raw = (uint16_t)pack_halves(f[0], 0.0f, T{});
     } else {
@@ -341,12 +339,11 @@ __device__ void fill_rows(const Rows& rows, int pieces, const PlanView& p, const
 // Dispatch: a token is read once and stored to each of its rows.  blockDim.y tokens per CTA, blockDim.x threads over
 // the row's pieces.
 // ---------------------------------------------------------------------------------------
-constexpr int kUnroll = 4;
-
 template <typename P>
 __device__ __forceinline__ void copy_token(const uint8_t* src, const Rows& rows, const int (&row)[kMaxTopK], int K, int pieces, int begin,
                                            int step)
 {
+    constexpr int kUnroll = P::kBytes == 16 ? 4 : 8;
     for (int i0 = begin; i0 < pieces; i0 += step * kUnroll) {
         P v[kUnroll];
 #pragma unroll
@@ -642,9 +639,28 @@ int check_apart(const Call& call, const Extent& written, const Extent& other)
     return share_memory(written, other) ? call.bad("%s and %s share memory", written.name, other.name) : MOE_FP8_B200_OK;
 }
 
-bool on_16_bytes(const Extent& e)
+// The widest piece, up to 16 bytes, that the rows of both matrices consist of.
+int piece_bytes(const Extent& a, const Extent& b, const Extent& c = {})
 {
-    return !e.base || (((uintptr_t)e.base | (uintptr_t)e.row_bytes | (e.rows > 1 ? (uintptr_t)e.stride_bytes : 0)) & 15u) == 0;
+    uintptr_t all = 16;
+    for (const Extent* e : {&a, &b, &c})
+        if (e->base) all |= (uintptr_t)e->base | (uintptr_t)e->row_bytes | (e->rows > 1 ? (uintptr_t)e->stride_bytes : 0);
+    return (int)(all & (~all + 1));
+}
+
+// f(type, elements of a piece)
+template <typename F>
+cudaError_t with_pieces(int dtype, int bytes, F f)
+{
+    auto of = [&](auto type) {
+        typedef decltype(type) T;
+        if constexpr (sizeof(T) == 2)
+            if (bytes == 2) return f(type, std::integral_constant<int, 1>{});
+        return bytes == 16  ? f(type, std::integral_constant<int, 16 / sizeof(T)>{})
+               : bytes == 8 ? f(type, std::integral_constant<int, 8 / sizeof(T)>{})
+                            : f(type, std::integral_constant<int, 4 / sizeof(T)>{});
+    };
+    return dtype == MOE_FP8_B200_BF16 ? of(__nv_bfloat16{}) : dtype == MOE_FP8_B200_FP16 ? of(__half{}) : of(float{});
 }
 
 Rows as_rows(const Extent& e) { return {static_cast<uint8_t*>(const_cast<void*>(e.base)), e.stride_bytes}; }
@@ -728,8 +744,7 @@ cudaError_t enqueue_dispatch(const void* ids, int id_bits, int64_t first, const 
                              const PlanView& p, int zero_unused, cudaStream_t stream)
 {
     const Fill fill = fill_for(p, zero_unused);
-    const bool wide = on_16_bytes(x) && on_16_bytes(rows);
-    auto with = [&](auto type, auto n) {
+    return with_pieces(element_size(dtype) == 2 ? MOE_FP8_B200_FP16 : dtype, piece_bytes(x, rows), [&](auto type, auto n) {
         typedef decltype(type) T;
         constexpr int N = decltype(n)::value;
         if (ids && p.pairs <= kSmallPairs && p.T <= kSmallTokens && p.E <= kSmallThreads)
@@ -737,10 +752,7 @@ cudaError_t enqueue_dispatch(const void* ids, int id_bits, int64_t first, const 
                                  : launch_small<int64_t, T, N>(ids, first, x, rows, p, fill, stream);
         const cudaError_t e = ids ? enqueue_sort(ids, id_bits, first, p, stream) : cudaSuccess;
         return e == cudaSuccess ? launch_dispatch<T, N>(x, rows, p, fill, stream) : e;
-    };
-    if (element_size(dtype) == 4)
-        return wide ? with(float{}, std::integral_constant<int, 4>{}) : with(float{}, std::integral_constant<int, 1>{});
-    return wide ? with(__half{}, std::integral_constant<int, 8>{}) : with(__half{}, std::integral_constant<int, 1>{});
+    });
 }
 
 template <typename T, int N>
@@ -840,18 +852,9 @@ int moe_fp8_b200_combine_rows(const void* y, int64_t y_stride, const float* weig
     if (rc == MOE_FP8_B200_OK && weights) rc = check_apart(call, eo, {"weights", weights, 1, 4ll * p.pairs, 0});
     if (rc != MOE_FP8_B200_OK) return rc;
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
-    const bool wide = on_16_bytes(ey) && on_16_bytes(eo);
-    switch (dtype) {
-        case MOE_FP8_B200_BF16:
-            return call.cuda(wide ? launch_combine_rows<__nv_bfloat16, 8>(ey, weights, eo, p, s)
-                                  : launch_combine_rows<__nv_bfloat16, 1>(ey, weights, eo, p, s));
-        case MOE_FP8_B200_FP16:
-            return call.cuda(wide ? launch_combine_rows<__half, 8>(ey, weights, eo, p, s)
-                                  : launch_combine_rows<__half, 1>(ey, weights, eo, p, s));
-        default:
-            return call.cuda(wide ? launch_combine_rows<float, 4>(ey, weights, eo, p, s)
-                                  : launch_combine_rows<float, 1>(ey, weights, eo, p, s));
-    }
+    return call.cuda(with_pieces(dtype, piece_bytes(ey, eo), [&](auto type, auto n) {
+        return launch_combine_rows<decltype(type), decltype(n)::value>(ey, weights, eo, p, s);
+    }));
 }
 
 int moe_fp8_b200_combine_rows_backward(const void* grad_out, int64_t grad_out_stride, const void* y, int64_t y_stride,
@@ -883,18 +886,9 @@ int moe_fp8_b200_combine_rows_backward(const void* grad_out, int64_t grad_out_st
     }
     if (rc != MOE_FP8_B200_OK) return rc;
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
-    const bool wide = on_16_bytes(eg) && on_16_bytes(ey) && on_16_bytes(ed);
-    switch (dtype) {
-        case MOE_FP8_B200_BF16:
-            return call.cuda(wide ? launch_combine_grad<__nv_bfloat16, 8>(eg, ey, weights, ed, grad_weights, p, zero_unused, s)
-                                  : launch_combine_grad<__nv_bfloat16, 1>(eg, ey, weights, ed, grad_weights, p, zero_unused, s));
-        case MOE_FP8_B200_FP16:
-            return call.cuda(wide ? launch_combine_grad<__half, 8>(eg, ey, weights, ed, grad_weights, p, zero_unused, s)
-                                  : launch_combine_grad<__half, 1>(eg, ey, weights, ed, grad_weights, p, zero_unused, s));
-        default:
-            return call.cuda(wide ? launch_combine_grad<float, 4>(eg, ey, weights, ed, grad_weights, p, zero_unused, s)
-                                  : launch_combine_grad<float, 1>(eg, ey, weights, ed, grad_weights, p, zero_unused, s));
-    }
+    return call.cuda(with_pieces(dtype, piece_bytes(eg, ey, ed), [&](auto type, auto n) {
+        return launch_combine_grad<decltype(type), decltype(n)::value>(eg, ey, weights, ed, grad_weights, p, zero_unused, s);
+    }));
 }
 
 }  // extern "C"

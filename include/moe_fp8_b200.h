@@ -460,7 +460,7 @@ MOE_FP8_B200_API int moe_fp8_b200_sort_tokens(const void* topk_idx, int id_bits,
 
 /* rows[r, :] = x[row_pair[r] / top_k, :] for the rows that have a pair, zeros for the padding; unused rows are left as
  * they were, or zeroed too with zero_unused != 0.  x is [T, hidden] with `x_stride` elements from row to row, rows [plan_rows, hidden] with `rows_stride`.
- * Rows whose addresses and length are multiples of 16 bytes move in 16-byte pieces, others element by element.
+ * Rows move in the widest pieces of 16, 8, 4 or 2 bytes that their addresses and length are multiples of.
  * The plan must be one that moe_fp8_b200_sort_tokens filled for these sizes. */
 MOE_FP8_B200_API int moe_fp8_b200_dispatch_rows(const void* x, int64_t x_stride, void* rows, int64_t rows_stride, int dtype,
                                                 int hidden, const moe_fp8_b200_plan* plan, int zero_unused, void* stream,
