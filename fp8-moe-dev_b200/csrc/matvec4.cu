@@ -54,6 +54,7 @@ constexpr int kRowsOfX = 8;                   // rows of x that share a read of 
 constexpr int kMaxBlocks = 16;                // 32-column blocks of a warp
 constexpr int kFewRows = 4;                   // rows of x up to which the product goes by integers
 constexpr int kMaxK = 8192;
+constexpr int kMaxRows = 1 << 21;              // whatever a plan says, the sums over its experts stay within 32 bits
 constexpr int kMaxStages = 4;
 constexpr uint32_t kSwizzleAtom = 1024;        // what the swizzle repeats after
 constexpr int kMaxExperts = MOE_FP8_B200_PLAN_MAX_EXPERTS;
@@ -632,6 +633,8 @@ __global__ void __launch_bounds__(kThreads, 1) matvec4_kernel(const MatvecArgs a
     const int tiles = a.N / kTileRows;
     constexpr int per_stage = kWarps / SPLIT;
     if (threadIdx.x == 0) {
+        // a plan whose experts' rows overlap is none: nothing is done
+        if (ex.first[a.E] > a.rows / kRowsOfX + a.E) ex.first[a.E] = ex.cost[a.E] = 0;
         const unsigned begin = unit_at_share(ex, a, blockIdx.x, tiles), end = unit_at_share(ex, a, blockIdx.x + 1, tiles);
         sh.begin = begin;
         sh.end = end;
@@ -895,6 +898,7 @@ extern "C" int moe_fp8_b200_matvec_w4(const void* x, int64_t x_stride, int by_to
     }
     if (rows < 0) return bad("num_rows %d < 0", num_rows);
     if (rows == 0) return MOE_FP8_B200_OK;
+    if (rows > kMaxRows) return bad("%lld rows are more than %d", (long long)rows, kMaxRows);
     if ((rows / kRowsOfX + w->num_experts + 1) * kManyCost * (w->n / kTileRows) >= ((int64_t)1 << 31))
         return bad("%lld rows by n = %d are too many for a product of a small batch", (long long)rows, w->n);
     int dev = 0, sms = 0;

@@ -8,7 +8,10 @@ the experts' rows back at their tokens with the routing weights applied, and the
 
 `sort_and_dispatch` is the first two in one call.  `dispatch` and `combine` take part in autograd; `dispatch_backward`
 and `combine_backward` are their gradients as plain calls.  Results go to the tensors passed for them, or to new ones.
-Everything runs on the current stream of the tensors' device and returns without synchronising.  The counterparts
+Everything runs on the current stream of the tensors' device, returns without synchronising and may be captured into a
+graph.  (A captured backward pass follows torch's own rule: no other graph of the same leaves may be alive, since the nodes that
+accumulate their gradients belong to the stream that made them.  The `_backward` functions have no such rule.)  `matvec_w4`
+is the experts' product of a decode batch with 4-bit weights.  The counterparts
 inside the reference's layer are kernel/moe_fp8.cu:1064-1115 (permute) and :2254-2323 (combine).
 """
 from __future__ import annotations
@@ -124,7 +127,7 @@ class ExpertPlan:
 
     Made by sort_tokens, or from four tensors of one's own (to be filled, or filled elsewhere)."""
     __slots__ = ("pair_row", "row_pair", "expert_offset", "expert_count", "align", "num_tokens", "top_k", "num_experts",
-                 "capacity", "device", "index", "_c")
+                 "capacity", "device", "index", "_c", "_filled")
 
     def __init__(self, pair_row, row_pair, expert_offset, expert_count, *, align: int = 1):
         index = _on_gpu("pair_row", pair_row)
@@ -136,6 +139,7 @@ class ExpertPlan:
         self.capacity = capacity = plan_rows(T, K, E, align)
         self.pair_row, self.row_pair, self.expert_offset, self.expert_count = pair_row, row_pair, expert_offset, expert_count
         self.device, self.index = pair_row.device, index
+        self._filled = 0   # how often it was filled: a backward pass wants the plan of its forward pass
         i32 = torch.int32
         self._c = C.byref(_lib.Plan(T, K, E, align, _packed("pair_row", pair_row, i32, (T, K), index),
                                     _packed("row_pair", row_pair, i32, (capacity,), index),
@@ -182,6 +186,7 @@ def sort_tokens(topk_idx, num_experts: int, *, first_expert: int = 0, align: int
     """Sorts the (token, expert) pairs of topk_idx [T, top_k] (int32 or int64) by expert.  The plan's experts are
     [first_expert, first_expert + num_experts); pairs of other experts (an id of -1, another GPU's expert) have no row."""
     plan = _ids(topk_idx, num_experts, align, plan)
+    plan._filled += 1
     _call(_lib.load().moe_fp8_b200_sort_tokens, plan.index, topk_idx.data_ptr(), _ID_BITS[topk_idx.dtype], first_expert,
           plan._c)
     return plan
@@ -224,6 +229,7 @@ def sort_and_dispatch(x, topk_idx, num_experts: int, *, first_expert: int = 0, a
     if _wants_grad(x):
         return dispatch(x, sort_tokens(topk_idx, num_experts, first_expert=first_expert, align=align, plan=plan), rows), plan
     rows, args = _rows_for(x, plan, rows)
+    plan._filled += 1
     _call(_lib.load().moe_fp8_b200_sort_and_dispatch, plan.index, topk_idx.data_ptr(), _ID_BITS[topk_idx.dtype], first_expert,
           *args)
     return rows, plan
@@ -339,22 +345,28 @@ def _plain_rows(grad):
     return grad if grad.stride(1) == 1 else grad.contiguous()
 
 
+def _same_plan(ctx):
+    if ctx.plan._filled != ctx.filled:
+        raise RuntimeError("the plan was filled anew since the forward pass: keep one plan per pass")
+    return ctx.plan
+
+
 class _Dispatch(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, plan):
-        ctx.plan = plan
+        ctx.plan, ctx.filled = plan, plan._filled
         return dispatch(x.detach(), plan)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad_rows):
-        return dispatch_backward(_plain_rows(grad_rows), ctx.plan), None
+        return dispatch_backward(_plain_rows(grad_rows), _same_plan(ctx)), None
 
 
 class _Combine(torch.autograd.Function):
     @staticmethod
     def forward(ctx, y, weights, plan):
-        ctx.plan = plan
+        ctx.plan, ctx.filled = plan, plan._filled
         ctx.save_for_backward(y, weights)
         return _combine(y.detach(), weights.detach(), plan, None)
 
@@ -362,6 +374,6 @@ class _Combine(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad_out):
         y, weights = ctx.saved_tensors
-        grad_y, grad_weights = combine_backward(_plain_rows(grad_out), y, weights, ctx.plan,
+        grad_y, grad_weights = combine_backward(_plain_rows(grad_out), y, weights, _same_plan(ctx),
                                                 need_y=ctx.needs_input_grad[0], need_weights=ctx.needs_input_grad[1])
         return grad_y, grad_weights, None

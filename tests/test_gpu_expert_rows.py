@@ -324,6 +324,54 @@ def test_graph_replays_see_new_contents(pkg):
         check_plan(pkg, plan, ids, E, 0, align)
 
 
+def test_autograd_in_a_graph(pkg):
+    """Forward and backward captured together, after warm-up on a side stream, replayed with other contents."""
+    T, K, E, H = 50, 4, 16, 96
+    ids = some_ids(T, K, E, 41)
+    x = torch.randn(T, H, device="cuda", requires_grad=True)
+    w = torch.rand(T, K, device="cuda", requires_grad=True)
+    up = torch.randn(T, H, device="cuda")
+
+    def step():
+        rows, plan = pkg.sort_and_dispatch(x, ids, E)
+        (pkg.combine(rows * 2.0, w, plan) * up).sum().backward()
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            x.grad = w.grad = None
+            step()
+    torch.cuda.current_stream().wait_stream(side)
+    x.grad = w.grad = None
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    with torch.no_grad():
+        x.copy_(torch.randn(T, H, device="cuda"))
+        w.copy_(torch.rand(T, K, device="cuda"))
+        ids.copy_(some_ids(T, K, E, 42))
+    graph.replay()
+    torch.cuda.synchronize()
+    # every pair has a row: out = sum of the weights times 2x
+    want_x = 2.0 * up.double() * w.detach().double().sum(1, keepdim=True)
+    want_w = (2.0 * up.double() * x.detach().double()).sum(1, keepdim=True).expand(T, K)
+    # a product, K additions and two more products in fp32; a sum of H products against the sum of their magnitudes
+    assert bool(((x.grad.double() - want_x).abs() <= (K + 4) * 2.0 ** -24 * want_x.abs()).all())
+    mag = (2.0 * up.double() * x.detach().double()).abs().sum(1, keepdim=True)
+    assert bool(((w.grad.double() - want_w).abs() <= (H / 32 + 32 + 13 + 2) * 2.0 ** -24 * mag).all())
+
+
+def test_a_plan_filled_anew_before_the_backward_pass(pkg):
+    T, K, E, H = 8, 2, 4, 16
+    plan = pkg.ExpertPlan.empty(T, K, E)
+    x = torch.randn(T, H, device="cuda", requires_grad=True)
+    rows, _ = pkg.sort_and_dispatch(x, some_ids(T, K, E, 1), E, plan=plan)
+    pkg.sort_tokens(some_ids(T, K, E, 2), E, plan=plan)
+    with pytest.raises(RuntimeError, match="filled anew"):
+        rows.sum().backward()
+
+
 def test_another_stream(pkg):
     T, K, E, H = 2000, 8, 64, 1024
     ids = some_ids(T, K, E, 31)

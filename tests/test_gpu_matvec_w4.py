@@ -256,6 +256,26 @@ def test_a_decode_step(pkg):
         check()
 
 
+def test_a_plan_of_nonsense_reads_and_writes_nothing_outside(pkg):
+    """Offsets and counts that no sort gives: rows outside the matrices, experts on top of one another."""
+    T, K, E, N, C = 40, 2, 8, 32, 128
+    codes, scales, _ = make_weights((E,), N, C, 64, torch.bfloat16, False, 3)
+    for by_token in (False, True):
+        plan = pkg.sort_tokens(routed(T, K, E, 5), E)
+        plan.expert_offset[2], plan.expert_count[2] = -5, 3
+        plan.expert_offset[3], plan.expert_count[3] = plan.capacity + 7, 2
+        plan.expert_count[4] = 2**31 - 1
+        plan.row_pair[:4] = torch.tensor([-1, 2**31 - 1, -2**31, T * K], dtype=torch.int32, device="cuda")
+        x = torch.randn(T if by_token else plan.capacity, C, device="cuda").to(torch.bfloat16)
+        guard = torch.full((plan.capacity + 64, N), 3.0, dtype=torch.bfloat16, device="cuda")
+        pkg.matvec_w4(x, codes, scales, plan=plan, by_token=by_token, out=guard[32:32 + plan.capacity])
+        plan.expert_offset.fill_(0)
+        plan.expert_count.fill_(2**31 - 1)
+        pkg.matvec_w4(x, codes, scales, plan=plan, by_token=by_token, out=guard[32:32 + plan.capacity])
+        torch.cuda.synchronize()
+        assert bool((guard[:32] == 3).all()) and bool((guard[32 + plan.capacity:] == 3).all())
+
+
 def test_refusals(pkg):
     M, N, K, group = 4, 32, 256, 64
     codes, scales, z = make_weights((), N, K, group, torch.bfloat16, True, 1)

@@ -17,7 +17,8 @@ def call(pkg, n=32, k=256, group=64, E=1, dtype=0, gated=0, zeros=None, by_token
     (dict(dtype=2), "bf16 or fp16"), (dict(group=16), "group"), (dict(group=256), "group"), (dict(k=96), "multiple"),
     (dict(k=0), "multiple"), (dict(k=8256), "8192"), (dict(n=24), "multiple of 16"), (dict(n=0), "multiple of 16"),
     (dict(n=(1 << 20) + 16), "2^20"), (dict(E=0), "num_experts"), (dict(E=1025), "num_experts"), (dict(E=2), "plan"),
-    (dict(by_token=1), "plan"), (dict(rows=-1), "num_rows"), (dict(k=192, gated=1, zeros=16), "even number of groups")])
+    (dict(by_token=1), "plan"), (dict(rows=-1), "num_rows"), (dict(rows=(1 << 21) + 1), "rows are more"),
+    (dict(rows=1 << 21, n=1 << 20), "too many"), (dict(k=192, gated=1, zeros=16), "even number of groups")])
 def test_sizes(pkg, bad, text):
     rc, msg = call(pkg, **bad)
     assert rc == pkg._lib.ERR_INVALID_ARGUMENT and text in msg, msg
