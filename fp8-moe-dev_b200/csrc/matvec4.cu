@@ -259,11 +259,23 @@ template <> struct Half2<__half> {
     static __device__ __forceinline__ __half round(float v) { return __float2half_rn(v); }
 };
 
-__device__ __forceinline__ void mma_s8(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-    asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-        : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
-        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+__device__ __forceinline__ void mma_s8(int (&d)[4], const int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                       uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %12, %13};"
+        : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "r"(c[0]), "r"(c[1]), "r"(c[2]), "r"(c[3]));
 }
+// The start of every sum by integers (see ByInteger).  With a scale per block there are so many that it is kept in four registers
+// (16 tokens, groups of 32 with zero points: 63 us, 67 with four moves per sum); with one per pair the registers are worth
+// more (one token, 256 experts: 39 us, 41 with Ones).
+constexpr int kOne = 0x4b400000;
+struct Ones {
+    int v[4];
+    __device__ __forceinline__ Ones() {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) asm volatile("mov.b32 %0, %1;" : "=r"(v[i]) : "n"(kOne));
+    }
+};
 // (a ^ b) & mask in one instruction
 __device__ __forceinline__ uint32_t xor_and(uint32_t a, uint32_t b, uint32_t mask) {
     uint32_t d;
@@ -319,7 +331,7 @@ template <typename H, bool FINE, bool ZEROS, int SPLIT>
 struct ByType {
     static constexpr int kAtOnce = 1;
     template <int FIRST, int COUNT>
-    static __device__ __forceinline__ void multiply(float (&acc)[8], const uint32_t (&xr)[kMaxBlocks][4], const MatvecArgs& a, const TileView& v) {
+    static __device__ __forceinline__ void multiply(float (&acc)[8], const uint32_t (&xr)[kMaxBlocks][4], const Ones& ones, const MatvecArgs& a, const TileView& v) {
         constexpr int kScales = FINE ? 2 : 1, kBlocks = 2 / kScales;   // scales of a pair, blocks of a scale
         const Words<SPLIT, COUNT> w(v, FIRST);
 #pragma unroll
@@ -351,9 +363,8 @@ struct ByType {
 template <typename H, bool FINE, bool ZEROS, int SPLIT, int MMAS>
 struct ByInteger {
     static constexpr int kAtOnce = MMAS == 1 ? 2 : 1;
-    static constexpr int kOne = 0x4b400000;
     template <int FIRST, int COUNT>
-    static __device__ __forceinline__ void multiply(float (&acc)[8], const uint32_t (&xr)[kMaxBlocks][4], const MatvecArgs& a, const TileView& v) {
+    static __device__ __forceinline__ void multiply(float (&acc)[8], const uint32_t (&xr)[kMaxBlocks][4], const Ones& ones, const MatvecArgs& a, const TileView& v) {
         constexpr int kScales = FINE ? 2 : 1, kBlocks = 2 / kScales;
         const Words<SPLIT, COUNT> w(v, FIRST);
 #pragma unroll
@@ -361,10 +372,12 @@ struct ByInteger {
 #pragma unroll
             for (int i = 0; i < kScales; ++i) {
                 const Scales<H, ZEROS> s(a, v, FIRST + p, i != 0);
-                const uint32_t neg0 = (0u - s.z0 & 0xffu) * 0x01010101u, neg1 = (0u - s.z1 & 0xffu) * 0x01010101u;   // bytes -zero
+                const uint32_t neg0 = __byte_perm(0u - s.z0, 0, 0), neg1 = __byte_perm(0u - s.z1, 0, 0);   // bytes -zero
                 int c[MMAS][4];
+                if (!FINE) {
 #pragma unroll
-                for (int m = 0; m < MMAS; ++m) c[m][0] = c[m][1] = c[m][2] = c[m][3] = kOne;
+                    for (int m = 0; m < MMAS; ++m) c[m][0] = c[m][1] = c[m][2] = c[m][3] = kOne;
+                }
 #pragma unroll
                 for (int j = 2 * p + i * kBlocks; j < 2 * p + (i + 1) * kBlocks; ++j) {
                     const uint32_t(&x)[4] = xr[2 * FIRST + j];
@@ -378,8 +391,9 @@ struct ByInteger {
                     }
 #pragma unroll
                     for (int m = 0; m < MMAS; ++m) {
-                        mma_s8(c[m], even0, even1, odd0, odd1, x[2 * m], x[2 * m + 1]);
-                        if (ZEROS) mma_s8(c[m], neg0, neg1, neg0, neg1, x[2 * m], x[2 * m + 1]);
+                        if (FINE) mma_s8(c[m], ones.v, even0, even1, odd0, odd1, x[2 * m], x[2 * m + 1]);
+                        else mma_s8(c[m], c[m], even0, even1, odd0, odd1, x[2 * m], x[2 * m + 1]);
+                        if (ZEROS) mma_s8(c[m], c[m], neg0, neg1, neg0, neg1, x[2 * m], x[2 * m + 1]);
                     }
                 }
 #pragma unroll
@@ -393,14 +407,14 @@ struct ByInteger {
 
 // All of a warp's pairs, two at a time where the registers allow it.
 template <typename P, int FIRST = 0>
-__device__ __forceinline__ void multiply_pairs(float (&acc)[8], const uint32_t (&xr)[kMaxBlocks][4], const MatvecArgs& a, const TileView& v)
+__device__ __forceinline__ void multiply_pairs(float (&acc)[8], const uint32_t (&xr)[kMaxBlocks][4], const Ones& ones, const MatvecArgs& a, const TileView& v)
 {
     if constexpr (2 * FIRST < kMaxBlocks) {
         if (v.blocks > 2 * (FIRST + P::kAtOnce - 1)) {
-            P::template multiply<FIRST, P::kAtOnce>(acc, xr, a, v);
-            multiply_pairs<P, FIRST + P::kAtOnce>(acc, xr, a, v);
+            P::template multiply<FIRST, P::kAtOnce>(acc, xr, ones, a, v);
+            multiply_pairs<P, FIRST + P::kAtOnce>(acc, xr, ones, a, v);
         } else if (v.blocks > 2 * FIRST) {
-            P::template multiply<FIRST, 1>(acc, xr, a, v);
+            P::template multiply<FIRST, 1>(acc, xr, ones, a, v);
         }
     }
 }
@@ -746,6 +760,7 @@ __global__ void __launch_bounds__(kThreads, 1) matvec4_kernel(const MatvecArgs a
         const int pairs = ((a.K + 63) / 64 - member + SPLIT - 1) / SPLIT;
         view.blocks = pairs > 0 ? min(2 * pairs, a.K / 32 - 2 * (member + (pairs - 1) * SPLIT) + 2 * (pairs - 1)) : 0;
     }
+    const Ones ones;
     uint32_t xr[kMaxBlocks][4];
     int form = 0;                      // 0 in the type itself, 1 by integers for up to two rows, 2 for up to four
     float* const unit = sh.unit[warp];
@@ -776,9 +791,9 @@ __global__ void __launch_bounds__(kThreads, 1) matvec4_kernel(const MatvecArgs a
             TileView v = view;
             const int at = slot * a.stage_bytes;
             v.ring += at;
-            if (form == 1) multiply_pairs<ByInteger<H, FINE, ZEROS, SPLIT, 1>>(acc, xr, a, v);
-            else if (form == 2) multiply_pairs<ByInteger<H, FINE, ZEROS, SPLIT, 2>>(acc, xr, a, v);
-            else multiply_pairs<ByType<H, FINE, ZEROS, SPLIT>>(acc, xr, a, v);
+            if (form == 1) multiply_pairs<ByInteger<H, FINE, ZEROS, SPLIT, 1>>(acc, xr, ones, a, v);
+            else if (form == 2) multiply_pairs<ByInteger<H, FINE, ZEROS, SPLIT, 2>>(acc, xr, ones, a, v);
+            else multiply_pairs<ByType<H, FINE, ZEROS, SPLIT>>(acc, xr, ones, a, v);
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(smem_u32(&sh.empty_bar[slot]));
