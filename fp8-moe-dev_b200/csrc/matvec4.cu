@@ -15,13 +15,13 @@
 // What the SM has to do per byte of codes decides whether the stream runs at full rate (at 6.4 TB/s an SM gets 46 codes a
 // clock).  Two forms of the product:
 //
-// * Up to four rows of x, by integers (m16n8k32, s8).  A code becomes a signed byte with a shift and a mask per four:
+// * Up to four rows of x (two with zero points), by integers (m16n8k32, s8).  A code becomes a signed byte with a shift and a mask per four:
 //   (code - 8) * 16 sits in the upper half of a byte already, once its top bit is flipped; with zero points the code stays
 //   in the lower half and a second product takes the zero point off.  x is split, per row and warp, into four signed
 //   bytes of a 31-bit fixed-point number below the power of two above its largest value (exact for all values down to
 //   2^-23 of that, and off by 2^-31 of it below): four columns of the product per row, so two rows per instruction.
 //   The sums of a scale's products are exact integers, and become floats by starting from 1.5 * 2^23's bit pattern.
-// * Five to eight rows, or a row with an infinity or NaN, in the type itself (m16n8k16): 0x4300 | code is 128 + code in
+// * More rows, or a row with an infinity or NaN, in the type itself (m16n8k16): 0x4300 | code is 128 + code in
 //   bf16 (0x6400 | code is 1024 + code in fp16), exactly, and so is the difference to 128 + zero.  11 (9) operations
 //   per eight codes instead of 3.
 //
@@ -52,7 +52,10 @@ static_assert(kThreads * kLaunchRegisters == kWarps * 32 * kMultiplyRegisters + 
 constexpr int kTileRows = 16;                 // weight rows of a tile
 constexpr int kRowsOfX = 8;                   // rows of x that share a read of the weights
 constexpr int kMaxBlocks = 16;                // 32-column blocks of a warp
-constexpr int kFewRows = 4;                   // rows of x up to which the product goes by integers
+// Rows of x up to which the product goes by integers.  57344 x 7168 (212 MB), us by integers / in the type: 1 and 2 rows 51 / 62,
+// 3 and 4 rows 57 / 63, in fp16 59 / 60; groups of 32: 2 rows 57 / 70, in fp16 4 rows 65 / 64.  With zero points 2 rows 59 / 65,
+// with groups of 32 as well 65 / 70, but 4 rows 69 / 64 and 86 / 75: there an instruction per zero point adds up.
+__host__ __device__ constexpr int few_rows(bool zeros) { return zeros ? 2 : 4; }
 constexpr int kMaxK = 8192;
 constexpr int kMaxRows = 1 << 21;              // whatever a plan says, the sums over its experts stay within 32 bits
 constexpr int kMaxStages = 4;
@@ -134,15 +137,12 @@ __device__ __forceinline__ int last_at_or_below(const int* sums, int n, unsigned
     return lo;
 }
 
-// Tiles of up to eight rows, and what they cost: five to eight rows, in the type itself, take the SM a quarter longer than the
-// stream of their weights.
-constexpr int kFewCost = 4, kManyCost = 5;
-__host__ __device__ __forceinline__ int2 x_tiles_of(int rows) {
+// Tiles of up to eight rows, and what they cost: the figures at few_rows without what a call costs besides.
+constexpr int kTwoCost = 7, kFewCost = 8, kManyCost = 9;
+__device__ __forceinline__ int2 x_tiles_of(int rows, bool zeros) {
     const int full = rows / kRowsOfX, rest = rows % kRowsOfX;
-    int2 v;
-    v.x = full + (rest > 0);
-    v.y = full * kManyCost + (rest > kFewRows ? kManyCost : rest > 0 ? kFewCost : 0);
-    return v;
+    return make_int2(full + (rest > 0),
+                     full * kManyCost + (rest > few_rows(zeros) ? kManyCost : rest > 2 ? kFewCost : rest > 0 ? kTwoCost : 0));
 }
 
 // First unit (a tile of weights for a tile of x rows, in Run's order) of CTA `share`: the CTAs get equal costs.  The host sees
@@ -605,7 +605,7 @@ __global__ void __launch_bounds__(kThreads, 1) matvec4_kernel(const MatvecArgs a
             if (e < a.E) {
                 const int off = e0 ? a.expert_offset[e] : mine.x, count = e0 ? a.expert_count[e] : mine.y;
                 const int2 rows = off >= 0 && count > 0 && off < a.rows ? make_int2(off, min(count, a.rows - off)) : make_int2(0, 0);
-                own = x_tiles_of(rows.y);
+                own = x_tiles_of(rows.y, ZEROS);
                 ex.rows[e] = rows;
             }
             int2 upto = own;
@@ -635,7 +635,7 @@ __global__ void __launch_bounds__(kThreads, 1) matvec4_kernel(const MatvecArgs a
         }
     } else {
         if (threadIdx.x == 0) {
-            const int2 v = x_tiles_of(a.rows);
+            const int2 v = x_tiles_of(a.rows, ZEROS);
             ex.first[0] = ex.cost[0] = 0;
             ex.first[1] = v.x;
             ex.cost[1] = v.y;
@@ -782,7 +782,7 @@ __global__ void __launch_bounds__(kThreads, 1) matvec4_kernel(const MatvecArgs a
         if (s.row != row) {
             row = s.row;
             form = 0;
-            if (s.rows <= kFewRows) form = load_digits<T, SPLIT>(xr, unit, a, row, s.rows, member, lane);
+            if (s.rows <= few_rows(ZEROS)) form = load_digits<T, SPLIT>(xr, unit, a, row, s.rows, member, lane);
             if (form == 0) load_values<T, SPLIT>(xr, unit, a, row, s.rows, member, lane);
         }
         if (it < 0) continue;
@@ -792,7 +792,7 @@ __global__ void __launch_bounds__(kThreads, 1) matvec4_kernel(const MatvecArgs a
             const int at = slot * a.stage_bytes;
             v.ring += at;
             if (form == 1) multiply_pairs<ByInteger<H, FINE, ZEROS, SPLIT, 1>>(acc, xr, ones, a, v);
-            else if (form == 2) multiply_pairs<ByInteger<H, FINE, ZEROS, SPLIT, 2>>(acc, xr, ones, a, v);
+            else if (!ZEROS && form == 2) multiply_pairs<ByInteger<H, FINE, false, SPLIT, 2>>(acc, xr, ones, a, v);
             else multiply_pairs<ByType<H, FINE, ZEROS, SPLIT>>(acc, xr, ones, a, v);
         }
         __syncwarp();

@@ -510,7 +510,7 @@ typedef struct moe_fp8_b200_w4 {
  * gated: the weights are n / 2 linear rows followed by n / 2 gated ones, as in gemm1_weights of moe_fp8_b200_args, and out
  * [.., n / 2] is silu(y[r, n / 2 + i]) * y[r, i] (with zero points the number of groups is then even).
  * For decode batches (at most 2^21 rows): the weights are read once per eight rows of an expert.  Up to four rows of an
- * expert go by exact integer products of x as 31-bit numbers below the power of two above the largest value of a row (in a
+ * expert (two with zero points) go by exact integer products of x as 31-bit numbers below the power of two above the largest value of a row (in a
  * sixteenth to a quarter of its columns), which differ from x by at most 2^-31 of that power.  A load that never comes (a
  * second) leaves NaN.  No handle, as for the plan's functions. */
 MOE_FP8_B200_API int moe_fp8_b200_matvec_w4(const void* x, int64_t x_stride, int by_token, const moe_fp8_b200_w4* w, int gated,
