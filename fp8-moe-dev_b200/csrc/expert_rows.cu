@@ -45,7 +45,7 @@ struct Rows {
 // The sort: a counting sort by expert that keeps the order of the pairs.  One cluster of CTAs, one launch: every warp
 // counts a contiguous range of pairs, a CTA's warps and then the cluster's CTAs are scanned per expert (the other CTAs'
 // counts through distributed shared memory), and each warp walks its range again, where a pair's rank among the
-// pairs of its expert in the same 32 comes from a match over the warp.
+// pairs of its expert in the same 32 comes from votes over the warp.
 // ---------------------------------------------------------------------------------------
 constexpr int kSortThreads = 1024;
 
@@ -596,6 +596,28 @@ struct Call {
     }
 };
 
+int check_apart(const Call& call, const Extent& written, const Extent& other)
+{
+    return share_memory(written, other) ? call.bad("%s and %s share memory", written.name, other.name) : MOE_FP8_B200_OK;
+}
+
+struct PlanExtents {
+    Extent a[4];
+    explicit PlanExtents(const PlanView& p)
+        : a{{"pair_row", p.pair_row, 1, 4ll * p.pairs, 0},
+            {"row_pair", p.row_pair, 1, 4ll * p.capacity, 0},
+            {"expert_offset", p.expert_offset, 1, 4ll * (p.E + 1), 0},
+            {"expert_count", p.expert_count, 1, 4ll * p.E, 0}} {}
+};
+
+int check_apart_from_plan(const Call& call, const Extent& other, const PlanView& p)
+{
+    const PlanExtents plan(p);
+    for (const Extent& e : plan.a)
+        if (share_memory(other, e)) return call.bad("%s and the plan's %s share memory", other.name, e.name);
+    return MOE_FP8_B200_OK;
+}
+
 int check_plan(Call& call, const moe_fp8_b200_plan* plan, PlanView& v)
 {
     if (!plan) return call.bad("plan is NULL");
@@ -603,6 +625,14 @@ int check_plan(Call& call, const moe_fp8_b200_plan* plan, PlanView& v)
     if (rows < 0)
         return call.bad("plan sizes out of range: num_tokens %d, top_k %d (1 .. %d), num_experts %d (1 .. %d), align %d (1 .. %d)",
                         plan->num_tokens, plan->top_k, kMaxTopK, plan->num_experts, kMaxExperts, plan->align, kMaxAlign);
+    v = {plan->num_tokens, plan->top_k, plan->num_experts, plan->align, plan->num_tokens * plan->top_k, (int)rows,
+         plan->pair_row, plan->row_pair, plan->expert_offset, plan->expert_count};
+    const PlanExtents arrays(v);
+    for (int i = 0; i < 4; ++i)
+        for (int j = i + 1; j < 4; ++j) {
+            const int rc = check_apart(call, arrays.a[i], arrays.a[j]);
+            if (rc != MOE_FP8_B200_OK) return rc;
+        }
     int rc = call.begin();
     if (rc == MOE_FP8_B200_OK && plan->num_tokens > 0) {
         rc = call.tensor("pair_row", plan->pair_row, 4);
@@ -610,10 +640,7 @@ int check_plan(Call& call, const moe_fp8_b200_plan* plan, PlanView& v)
     }
     if (rc == MOE_FP8_B200_OK) rc = call.tensor("expert_offset", plan->expert_offset, 4);
     if (rc == MOE_FP8_B200_OK) rc = call.tensor("expert_count", plan->expert_count, 4);
-    if (rc != MOE_FP8_B200_OK) return rc;
-    v = {plan->num_tokens, plan->top_k, plan->num_experts, plan->align, plan->num_tokens * plan->top_k, (int)rows,
-         plan->pair_row, plan->row_pair, plan->expert_offset, plan->expert_count};
-    return MOE_FP8_B200_OK;
+    return rc;
 }
 
 int element_size(int dtype)
@@ -632,11 +659,6 @@ int check_rows(const Call& call, const char* name, const void* p, int64_t stride
     const int rc = call.tensor(name, p, size);
     out = {name, p, rows, (int64_t)hidden * size, stride * size};
     return rc;
-}
-
-int check_apart(const Call& call, const Extent& written, const Extent& other)
-{
-    return share_memory(written, other) ? call.bad("%s and %s share memory", written.name, other.name) : MOE_FP8_B200_OK;
 }
 
 // The widest piece, up to 16 bytes, that the rows of both matrices consist of.
@@ -775,10 +797,12 @@ cudaError_t launch_combine_grad(const Extent& grad_out, const Extent& y, const f
                         weights, as_rows(grad_y), grad_weights, pieces, fill, p);
 }
 
-int check_ids(const Call& call, const void* ids, int id_bits)
+// The ids are read twice, by every CTA of the small kernel: the plan written over them would be read as ids.
+int check_ids(const Call& call, const void* ids, int id_bits, const PlanView& p)
 {
     if (id_bits != 32 && id_bits != 64) return call.bad("id_bits must be 32 or 64, got %d", id_bits);
-    return call.tensor("topk_idx", ids, id_bits / 8);
+    const int rc = call.tensor("topk_idx", ids, id_bits / 8);
+    return rc == MOE_FP8_B200_OK ? check_apart_from_plan(call, {"topk_idx", ids, 1, (int64_t)p.pairs * (id_bits / 8), 0}, p) : rc;
 }
 
 }  // namespace
@@ -799,7 +823,7 @@ int moe_fp8_b200_sort_tokens(const void* topk_idx, int id_bits, int64_t first_ex
     Call call{err, err_len};
     PlanView p;
     int rc = check_plan(call, plan, p);
-    if (rc == MOE_FP8_B200_OK && p.T > 0) rc = check_ids(call, topk_idx, id_bits);
+    if (rc == MOE_FP8_B200_OK && p.T > 0) rc = check_ids(call, topk_idx, id_bits, p);
     if (rc != MOE_FP8_B200_OK) return rc;
     return call.cuda(enqueue_sort(topk_idx, id_bits, first_expert, p, static_cast<cudaStream_t>(stream)));
 }
@@ -815,6 +839,7 @@ int moe_fp8_b200_dispatch_rows(const void* x, int64_t x_stride, void* rows, int6
     rc = check_rows(call, "x", x, x_stride, p.T, dtype, hidden, false, ex);
     if (rc == MOE_FP8_B200_OK) rc = check_rows(call, "rows", rows, rows_stride, p.capacity, dtype, hidden, true, er);
     if (rc == MOE_FP8_B200_OK) rc = check_apart(call, er, ex);
+    if (rc == MOE_FP8_B200_OK) rc = check_apart_from_plan(call, er, p);
     if (rc != MOE_FP8_B200_OK) return rc;
     return call.cuda(enqueue_dispatch(nullptr, 0, 0, ex, er, dtype, p, zero_unused, static_cast<cudaStream_t>(stream)));
 }
@@ -827,10 +852,16 @@ int moe_fp8_b200_sort_and_dispatch(const void* topk_idx, int id_bits, int64_t fi
     PlanView p;
     Extent ex, er;
     int rc = check_plan(call, plan, p);
-    if (rc == MOE_FP8_B200_OK && p.T > 0) rc = check_ids(call, topk_idx, id_bits);
+    if (rc == MOE_FP8_B200_OK && p.T > 0) rc = check_ids(call, topk_idx, id_bits, p);
     if (rc == MOE_FP8_B200_OK && p.T > 0) rc = check_rows(call, "x", x, x_stride, p.T, dtype, hidden, false, ex);
     if (rc == MOE_FP8_B200_OK && p.T > 0) rc = check_rows(call, "rows", rows, rows_stride, p.capacity, dtype, hidden, true, er);
-    if (rc == MOE_FP8_B200_OK && p.T > 0) rc = check_apart(call, er, ex);
+    if (rc == MOE_FP8_B200_OK && p.T > 0) {
+        Extent ei = {"topk_idx", topk_idx, 1, (int64_t)p.pairs * (id_bits / 8), 0};
+        for (const Extent* other : {&ex, &ei})
+            if (rc == MOE_FP8_B200_OK) rc = check_apart(call, er, *other);
+        for (const Extent* other : {&er, &ex})
+            if (rc == MOE_FP8_B200_OK) rc = check_apart_from_plan(call, *other, p);
+    }
     if (rc != MOE_FP8_B200_OK) return rc;
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
     return call.cuda(p.T > 0 ? enqueue_dispatch(topk_idx, id_bits, first_expert, ex, er, dtype, p, zero_unused, s)
@@ -849,6 +880,7 @@ int moe_fp8_b200_combine_rows(const void* y, int64_t y_stride, const float* weig
     if (rc == MOE_FP8_B200_OK) rc = check_rows(call, "out", out, out_stride, p.T, dtype, hidden, true, eo);
     if (rc == MOE_FP8_B200_OK && weights) rc = call.tensor("weights", weights, 4);
     if (rc == MOE_FP8_B200_OK) rc = check_apart(call, eo, ey);
+    if (rc == MOE_FP8_B200_OK) rc = check_apart_from_plan(call, eo, p);
     if (rc == MOE_FP8_B200_OK && weights) rc = check_apart(call, eo, {"weights", weights, 1, 4ll * p.pairs, 0});
     if (rc != MOE_FP8_B200_OK) return rc;
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
@@ -872,6 +904,7 @@ int moe_fp8_b200_combine_rows_backward(const void* grad_out, int64_t grad_out_st
     if (rc == MOE_FP8_B200_OK && grad_y) {
         rc = check_rows(call, "grad_y", grad_y, grad_y_stride, p.capacity, dtype, hidden, true, ed);
         if (rc == MOE_FP8_B200_OK) rc = check_apart(call, ed, eg);
+        if (rc == MOE_FP8_B200_OK) rc = check_apart_from_plan(call, ed, p);
         if (rc == MOE_FP8_B200_OK) rc = check_apart(call, ed, {"weights", weights, 1, 4ll * p.pairs, 0});
     }
     if (rc == MOE_FP8_B200_OK && grad_weights) {
@@ -880,6 +913,7 @@ int moe_fp8_b200_combine_rows_backward(const void* grad_out, int64_t grad_out_st
         const Extent dw = {"grad_weights", grad_weights, 1, 4ll * p.pairs, 0};
         if (rc == MOE_FP8_B200_OK) rc = check_apart(call, ed, ey);
         if (rc == MOE_FP8_B200_OK) rc = check_apart(call, dw, eg);
+        if (rc == MOE_FP8_B200_OK) rc = check_apart_from_plan(call, dw, p);
         if (rc == MOE_FP8_B200_OK) rc = check_apart(call, dw, ey);
         if (rc == MOE_FP8_B200_OK) rc = check_apart(call, dw, ed);
         if (rc == MOE_FP8_B200_OK) rc = check_apart(call, dw, {"weights", weights, 1, 4ll * p.pairs, 0});

@@ -938,7 +938,10 @@ extern "C" int moe_fp8_b200_matvec_w4(const void* x, int64_t x_stride, int by_to
     const Extent eo = {"out", out, rows, columns * 2, out_stride * 2}, ex = {"x", x, x_rows, (int64_t)w->k * 2, x_stride * 2};
     const int64_t all = (int64_t)w->num_experts * w->n;
     const Extent inputs[] = {ex, {"codes", w->codes, 1, all * (w->k / 2), 0}, {"scales", w->scales, 1, all * groups * 2, 0},
-                             {"zeros", w->zeros, 1, all * groups, 0}};
+                             {"zeros", w->zeros, 1, all * groups, 0},
+                             {"expert_offset", plan ? plan->expert_offset : nullptr, 1, 4ll * (w->num_experts + 1), 0},
+                             {"expert_count", plan ? plan->expert_count : nullptr, 1, 4ll * w->num_experts, 0},
+                             {"row_pair", plan && by_token ? plan->row_pair : nullptr, 1, 4ll * rows, 0}};
     for (const Extent& in : inputs)
         if (share_memory(eo, in)) return bad("out and %s share memory", in.name);
 

@@ -432,7 +432,8 @@ MOE_FP8_B200_API int moe_fp8_b200_route_noalloc(const float* routing_logits, con
  * within an expert by pair.  Expert e owns rows [expert_offset[e], expert_offset[e] + expert_count[e]); expert_offset[e + 1]
  * is its end rounded up so that the next expert starts a multiple of `align` rows further (128: the 128-row tiles of a
  * grouped GEMM never hold two experts).  The rows between are its padding, the rows behind
- * expert_offset[num_experts] are unused.  The caller owns the four arrays. */
+ * expert_offset[num_experts] are unused.  The caller owns the four arrays; they share no memory with one another, with the
+ * ids or with a result. */
 typedef struct moe_fp8_b200_plan {
     int32_t num_tokens;     /* T, 0 .. */
     int32_t top_k;          /* 1 .. MOE_FP8_B200_PLAN_MAX_TOP_K */
@@ -481,7 +482,8 @@ MOE_FP8_B200_API int moe_fp8_b200_combine_rows(const void* y, int64_t y_stride, 
 
 /* The gradients of moe_fp8_b200_combine_rows: grad_y[r, :] = weights[pair] * grad_out[token, :] (padding rows zero,
  * unused rows left as they were, or zeroed too with zero_unused != 0) and grad_weights[t, k] = <grad_out[t, :], y[pair_row[t, k], :]>, summed in fp32 in a fixed
- * order (0 for a pair without a row).  Either may be NULL if it is not wanted; y may be NULL with grad_weights. */
+ * order (0 for a pair without a row).  Either may be NULL if it is not wanted; y is read for grad_weights only,
+ * and may be NULL without it. */
 MOE_FP8_B200_API int moe_fp8_b200_combine_rows_backward(const void* grad_out, int64_t grad_out_stride, const void* y,
                                                         int64_t y_stride, const float* weights, void* grad_y,
                                                         int64_t grad_y_stride, float* grad_weights, int dtype, int hidden,

@@ -67,3 +67,16 @@ def test_binding_matches_the_header(pkg):
     for name in ("PLAN_MAX_TOP_K", "PLAN_MAX_EXPERTS"):
         assert int(re.search(rf"MOE_FP8_B200_{name} (\d+)", txt).group(1)) == getattr(L, name)
     assert C.sizeof(L.Plan) == 4 * 4 + 4 * 8
+
+
+@pytest.mark.parametrize("a,b", [(a, b) for a in range(4) for b in range(4) if a != b])
+def test_plan_arrays_that_share_memory(pkg, a, b):
+    """Refused before a pointer is looked at: the addresses belong to nothing."""
+    T, K, E, align = 4, 2, 8, 1
+    size = [4 * T * K, 4 * pkg.plan_rows(T, K, E, align), 4 * (E + 1), 4 * E]
+    at = [4096, 8192, 12288, 16384]
+    at[b] = at[a] + size[a] - 4   # the last element of a is the first of b
+    lib, err = pkg._lib.load(), C.create_string_buffer(256)
+    p = pkg._lib.Plan(T, K, E, align, *at)
+    assert lib.moe_fp8_b200_sort_tokens(1 << 20, 32, 0, C.byref(p), None, err, 256) == pkg._lib.ERR_INVALID_ARGUMENT
+    assert b"share memory" in err.value

@@ -424,3 +424,42 @@ def test_refusals_on_the_gpu(pkg):
     assert rc == pkg._lib.ERR_INVALID_ARGUMENT and b"current CUDA device" in err.value
     rc = pkg._lib.load().moe_fp8_b200_sort_tokens(ids.data_ptr(), 16, 0, plan._c, None, err, 256)
     assert rc == pkg._lib.ERR_INVALID_ARGUMENT and b"id_bits" in err.value
+
+
+@pytest.mark.parametrize("T", [4, 700])   # sorted and copied by one kernel, by two
+def test_plan_and_tensors_that_share_memory(pkg, T):
+    """Ids that the plan would be written over, and results that would be written over the plan."""
+    K, E, H = 2, 8, 64
+    ids = some_ids(T, K, E, 1)
+    plan = pkg.sort_tokens(ids, E)
+    want = [t.clone() for t in (plan.pair_row, plan.row_pair, plan.expert_offset, plan.expert_count)]
+    x = torch.randn(T, H, device="cuda")
+    rows = pkg.dispatch(x, plan)
+    w = torch.rand(T, K, device="cuda")
+    over_ids = pkg.ExpertPlan(ids, *(torch.empty_like(t) for t in (plan.row_pair, plan.expert_offset, plan.expert_count)))
+    by_row = pkg.ExpertPlan(torch.empty_like(ids), ids.view(-1), torch.empty_like(plan.expert_offset),
+                            torch.empty_like(plan.expert_count))
+    kept = ids.clone()
+    for p in (over_ids, by_row):
+        with pytest.raises(pkg.MoeError, match="topk_idx and the plan"):
+            pkg.sort_tokens(ids, E, plan=p)
+        with pytest.raises(pkg.MoeError, match="topk_idx and the plan"):
+            pkg.sort_and_dispatch(x, ids, E, plan=p)
+    # a plan within the memory of the results
+    memory = torch.zeros(T * K * H, device="cuda")
+    inside = pkg.ExpertPlan(memory[:T * K].view(torch.int32).view(T, K), torch.empty_like(plan.row_pair),
+                            torch.empty_like(plan.expert_offset), torch.empty_like(plan.expert_count))
+    pkg.sort_tokens(ids, E, plan=inside)
+    whole = memory.view(T * K, H)
+    for call in (lambda: pkg.dispatch(x, inside, rows=whole), lambda: pkg.sort_and_dispatch(x, ids, E, plan=inside, rows=whole),
+                 lambda: pkg.sort_and_dispatch(whole[:T], ids, E, plan=inside),
+                 lambda: pkg.combine(rows, w, inside, out=whole[:T]), lambda: pkg.dispatch_backward(rows, inside, out=whole[:T]),
+                 lambda: pkg.combine_backward(x, rows, w, inside, grad_y=whole),
+                 lambda: pkg.combine_backward(x, rows, w, inside, grad_weights=memory[:T * K].view(T, K))):
+        with pytest.raises(pkg.MoeError, match="share memory"):
+            call()
+    assert torch.equal(ids, kept) and torch.equal(inside.pair_row, want[0])
+    with pytest.raises(pkg.MoeError, match="rows and topk_idx share memory"):
+        mem = torch.zeros(T * K, H, device="cuda")
+        mine = mem.view(-1)[:T * K].view(torch.int32).view(T, K)
+        pkg.sort_and_dispatch(x, mine, E, rows=mem)

@@ -309,3 +309,19 @@ def test_refusals(pkg):
         with pytest.raises(error):
             call()
     assert pkg.matvec_w4(x[:0], codes, scales).shape == (0, N)
+
+
+def test_out_over_the_plan(pkg):
+    T, K, E, N, cols = 3, 2, 4, 16, 64
+    ids = torch.randint(0, E, (T, K), generator=torch.Generator().manual_seed(2)).int().cuda()
+    codes = torch.zeros(E, N, cols // 2, dtype=torch.uint8, device="cuda")
+    scales = torch.ones(E, N, 2, dtype=torch.bfloat16, device="cuda")
+    x = torch.ones(T, cols, dtype=torch.bfloat16, device="cuda")
+    for field, size in (("row_pair", T * K), ("expert_offset", E + 1), ("expert_count", E)):
+        memory = torch.zeros(T * K * N // 2, dtype=torch.int32, device="cuda")
+        arrays = dict(pair_row=(T, K), row_pair=(T * K,), expert_offset=(E + 1,), expert_count=(E,))
+        arrays = {k: torch.empty(v, dtype=torch.int32, device="cuda") for k, v in arrays.items()}
+        arrays[field] = memory[:size]
+        plan = pkg.sort_tokens(ids, E, plan=pkg.ExpertPlan(**arrays))
+        with pytest.raises(pkg.MoeError, match=f"out and {field} share memory"):
+            pkg.matvec_w4(x, codes, scales, plan=plan, by_token=True, out=memory.view(torch.bfloat16).view(T * K, N))
