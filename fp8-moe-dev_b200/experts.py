@@ -29,6 +29,7 @@ _ROW_TYPES = {torch.bfloat16: _lib.BF16, torch.float16: _lib.FP16, torch.float32
 _ID_BITS = {torch.int32: 32, torch.int64: 64}
 _raw_stream = torch._C._cuda_getCurrentRawStream
 _current_device = torch._C._cuda_getDevice
+_MAX_COLUMNS = 1 << 24
 _SMALL = 1 << 20   # tokens up to which a plan's size needs no word from the library
 
 
@@ -98,8 +99,8 @@ def _matrix(name, t, rows, columns, dtype, index):
 def _row_type(name, t):
     if t.dtype not in _ROW_TYPES:
         raise TypeError(f"{name} must be bfloat16, float16 or float32, got {t.dtype}")
-    if t.dim() != 2 or t.shape[1] < 1:
-        raise ValueError(f"{name} must be a matrix with at least one column, got shape {tuple(t.shape)}")
+    if t.dim() != 2 or not 1 <= t.shape[1] <= _MAX_COLUMNS:
+        raise ValueError(f"{name} must be a matrix of 1 .. {_MAX_COLUMNS} columns, got shape {tuple(t.shape)}")
     return _ROW_TYPES[t.dtype]
 
 
@@ -109,7 +110,8 @@ def plan_rows(num_tokens: int, top_k: int, num_experts: int, align: int = 1) -> 
     if 0 <= T <= _SMALL and 1 <= K <= _lib.PLAN_MAX_TOP_K and 1 <= E <= _lib.PLAN_MAX_EXPERTS and 1 <= align <= 1024:
         pairs = T * K
         return (pairs + min(E, pairs) * (align - 1) + align - 1) // align * align
-    rows = _lib.load().moe_fp8_b200_plan_rows(T, K, E, align)
+    # what passes 32 bits would reach the library cut to them
+    rows = _lib.load().moe_fp8_b200_plan_rows(T, K, E, align) if max(T, K, E, align) < 1 << 31 and min(T, K, E, align) >= 0 else -1
     if rows < 0:
         raise ValueError(f"no plan for {num_tokens} tokens, top_k {top_k} (1 .. {_lib.PLAN_MAX_TOP_K}), {num_experts} experts "
                          f"(1 .. {_lib.PLAN_MAX_EXPERTS}), align {align} (1 .. 1024)")
@@ -161,9 +163,11 @@ def _check_plan(plan):
     return plan.index
 
 
-def _ids(topk_idx, num_experts, align, plan):
+def _ids(topk_idx, num_experts, first_expert, align, plan):
     """The plan to fill for these ids."""
     index = _on_gpu("topk_idx", topk_idx)
+    if not -1 << 63 <= first_expert < 1 << 63:
+        raise ValueError(f"first_expert {first_expert} is not a 64-bit id")
     if topk_idx.dtype not in _ID_BITS:
         raise TypeError(f"topk_idx must be int32 or int64, got {topk_idx.dtype}")
     if topk_idx.dim() != 2:
@@ -185,7 +189,7 @@ def sort_tokens(topk_idx, num_experts: int, *, first_expert: int = 0, align: int
                 plan: Optional[ExpertPlan] = None) -> ExpertPlan:
     """Sorts the (token, expert) pairs of topk_idx [T, top_k] (int32 or int64) by expert.  The plan's experts are
     [first_expert, first_expert + num_experts); pairs of other experts (an id of -1, another GPU's expert) have no row."""
-    plan = _ids(topk_idx, num_experts, align, plan)
+    plan = _ids(topk_idx, num_experts, first_expert, align, plan)
     plan._filled += 1
     _call(_lib.load().moe_fp8_b200_sort_tokens, plan.index, topk_idx.data_ptr(), _ID_BITS[topk_idx.dtype], first_expert,
           plan._c)
@@ -225,7 +229,7 @@ def dispatch(x, plan: ExpertPlan, rows=None):
 def sort_and_dispatch(x, topk_idx, num_experts: int, *, first_expert: int = 0, align: int = 1,
                       plan: Optional[ExpertPlan] = None, rows=None) -> Tuple[torch.Tensor, ExpertPlan]:
     """sort_tokens and dispatch in one call: (rows, plan)."""
-    plan = _ids(topk_idx, num_experts, align, plan)
+    plan = _ids(topk_idx, num_experts, first_expert, align, plan)
     if _wants_grad(x):
         return dispatch(x, sort_tokens(topk_idx, num_experts, first_expert=first_expert, align=align, plan=plan), rows), plan
     rows, args = _rows_for(x, plan, rows)
@@ -326,10 +330,12 @@ def matvec_w4(x, codes, scales, *, zeros=None, plan: Optional[ExpertPlan] = None
     N, G = codes.shape[-2], scales.shape[-1]
     if G < 1 or K % G or K % 2:
         raise ValueError(f"scales of {G} groups do not divide {K} columns")
+    rows = x.shape[0] if plan is None else plan.capacity
+    if rows >= 1 << 31 or N >= 1 << 31:
+        raise ValueError(f"{rows} rows by {N} are too many")
     cp = _packed("codes", codes, torch.uint8, (*lead, N, K // 2), index)
     sp = _packed("scales", scales, x.dtype, (*lead, N, G), index)
     zp = None if zeros is None else _packed("zeros", zeros, torch.uint8, (*lead, N, G), index)
-    rows = x.shape[0] if plan is None else plan.capacity
     xp, xs = _matrix("x", x, plan.num_tokens if by_token else rows, K, x.dtype, index)
     columns = N // 2 if gated else N
     if out is None:

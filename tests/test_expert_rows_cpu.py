@@ -80,3 +80,12 @@ def test_plan_arrays_that_share_memory(pkg, a, b):
     p = pkg._lib.Plan(T, K, E, align, *at)
     assert lib.moe_fp8_b200_sort_tokens(1 << 20, 32, 0, C.byref(p), None, err, 256) == pkg._lib.ERR_INVALID_ARGUMENT
     assert b"share memory" in err.value
+
+
+@pytest.mark.parametrize("at", range(4))
+@pytest.mark.parametrize("wrap", [1 << 32, -(1 << 32), 1 << 64])
+def test_plan_sizes_beyond_32_bits(pkg, at, wrap):
+    sizes = [5, 8, 16, 4]
+    sizes[at] += wrap   # cut to 32 bits, a size that is allowed
+    with pytest.raises(ValueError, match="no plan"):
+        pkg.plan_rows(*sizes)

@@ -463,3 +463,20 @@ def test_plan_and_tensors_that_share_memory(pkg, T):
         mem = torch.zeros(T * K, H, device="cuda")
         mine = mem.view(-1)[:T * K].view(torch.int32).view(T, K)
         pkg.sort_and_dispatch(x, mine, E, rows=mem)
+
+
+def test_numbers_that_pass_their_bits(pkg):
+    ids = some_ids(4, 2, 8, 1)
+    x = torch.randn(4, 16, device="cuda")
+    for wrong in (dict(num_experts=8 + (1 << 32)), dict(num_experts=8, align=1 + (1 << 32)),
+                  dict(num_experts=8, first_expert=1 << 64), dict(num_experts=8, first_expert=-(1 << 63) - 1)):
+        with pytest.raises(ValueError):
+            pkg.sort_tokens(ids, **wrong)
+        with pytest.raises(ValueError):
+            pkg.sort_and_dispatch(x, ids, **wrong)
+    plan = pkg.sort_tokens(ids, 8)
+    wide = torch.empty(4, (1 << 32) + 16, device="meta")
+    for call in (lambda: pkg.dispatch(wide, plan), lambda: pkg.sort_and_dispatch(wide, ids, 8),
+                 lambda: pkg.dispatch_backward(wide, plan), lambda: pkg.combine(wide, torch.rand(4, 2, device="cuda"), plan)):
+        with pytest.raises(ValueError, match="columns"):
+            call()

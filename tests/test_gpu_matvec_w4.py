@@ -325,3 +325,14 @@ def test_out_over_the_plan(pkg):
         plan = pkg.sort_tokens(ids, E, plan=pkg.ExpertPlan(**arrays))
         with pytest.raises(pkg.MoeError, match=f"out and {field} share memory"):
             pkg.matvec_w4(x, codes, scales, plan=plan, by_token=True, out=memory.view(torch.bfloat16).view(T * K, N))
+
+
+def test_sizes_beyond_32_bits(pkg):
+    x = torch.zeros(1, 64, dtype=torch.bfloat16, device="cuda")
+    codes = torch.zeros(16, 32, dtype=torch.uint8, device="cuda")
+    scales = torch.ones(16, 2, dtype=torch.bfloat16, device="cuda")
+    with pytest.raises(ValueError, match="too many"):
+        pkg.matvec_w4(x.expand((1 << 32) + 1, 64), codes, scales)
+    with pytest.raises(ValueError, match="too many"):
+        pkg.matvec_w4(x, torch.empty((1 << 32) + 16, 32, dtype=torch.uint8, device="meta"),
+                      torch.empty((1 << 32) + 16, 2, dtype=torch.bfloat16, device="meta"))
