@@ -104,6 +104,15 @@ def _row_type(name, t):
     return _ROW_TYPES[t.dtype]
 
 
+def _result(name, t):
+    if isinstance(t, torch.Tensor) and _wants_grad(t):
+        raise ValueError(f"{name} requires a gradient: give a tensor that does not, or call under torch.no_grad()")
+
+
+# autograd learns that a given tensor was written: a backward pass that saved it raises instead of reading the new contents
+_written = torch._C._increment_version
+
+
 def plan_rows(num_tokens: int, top_k: int, num_experts: int, align: int = 1) -> int:
     """Rows that any choice of experts fits into: what `rows` of a dispatch must hold."""
     T, K, E, align = int(num_tokens), int(top_k), int(num_experts), int(align)
@@ -204,6 +213,8 @@ def _rows_for(x, plan, rows):
     fresh = rows is None
     if fresh:
         rows = torch.empty((plan.capacity, H), dtype=x.dtype, device=plan.device)
+    else:
+        _result("rows", rows)
     rp, rs = _matrix("rows", rows, plan.capacity, H, x.dtype, plan.index)
     return rows, (xp, xs, rp, rs, kind, H, plan._c, int(fresh))
 
@@ -223,6 +234,8 @@ def dispatch(x, plan: ExpertPlan, rows=None):
         return _Dispatch.apply(x, plan)
     rows, args = _rows_for(x, plan, rows)
     _call(_lib.load().moe_fp8_b200_dispatch_rows, plan.index, *args)
+    if not args[-1]:
+        _written((rows,))
     return rows
 
 
@@ -231,11 +244,15 @@ def sort_and_dispatch(x, topk_idx, num_experts: int, *, first_expert: int = 0, a
     """sort_tokens and dispatch in one call: (rows, plan)."""
     plan = _ids(topk_idx, num_experts, first_expert, align, plan)
     if _wants_grad(x):
-        return dispatch(x, sort_tokens(topk_idx, num_experts, first_expert=first_expert, align=align, plan=plan), rows), plan
+        if rows is not None:
+            raise ValueError("rows cannot be given where x requires a gradient")
+        return dispatch(x, sort_tokens(topk_idx, num_experts, first_expert=first_expert, align=align, plan=plan)), plan
     rows, args = _rows_for(x, plan, rows)
     plan._filled += 1
     _call(_lib.load().moe_fp8_b200_sort_and_dispatch, plan.index, topk_idx.data_ptr(), _ID_BITS[topk_idx.dtype], first_expert,
           *args)
+    if not args[-1]:
+        _written((rows,))
     return rows, plan
 
 
@@ -244,10 +261,15 @@ def _combine(y, weights, plan, out):
     H = y.shape[1]
     yp, ys = _matrix("y", y, plan.capacity, H, y.dtype, plan.index)
     wp = None if weights is None else _packed("weights", weights, torch.float32, (plan.num_tokens, plan.top_k), plan.index)
-    if out is None:
+    fresh = out is None
+    if fresh:
         out = torch.empty((plan.num_tokens, H), dtype=y.dtype, device=plan.device)
+    else:
+        _result("out", out)
     op, os = _matrix("out", out, plan.num_tokens, H, y.dtype, plan.index)
     _call(_lib.load().moe_fp8_b200_combine_rows, plan.index, yp, ys, wp, op, os, kind, H, plan._c)
+    if not fresh:
+        _written((out,))
     return out
 
 
@@ -285,13 +307,22 @@ def combine_backward(grad_out, y, weights, plan: ExpertPlan, grad_y=None, grad_w
     if need_y:
         if fresh:
             grad_y = torch.empty((plan.capacity, H), dtype=dtype, device=device)
+        else:
+            _result("grad_y", grad_y)
         dp, ds = _matrix("grad_y", grad_y, plan.capacity, H, dtype, index)
+    fresh_weights = grad_weights is None
     if need_weights:
-        if grad_weights is None:
+        if fresh_weights:
             grad_weights = torch.empty((plan.num_tokens, plan.top_k), dtype=torch.float32, device=device)
+        else:
+            _result("grad_weights", grad_weights)
         dwp = _packed("grad_weights", grad_weights, torch.float32, (plan.num_tokens, plan.top_k), index)
     _call(_lib.load().moe_fp8_b200_combine_rows_backward, index, gp, gs, yp, ys, wp, dp, ds, dwp, kind, H, plan._c,
           int(fresh))
+    if need_y and not fresh:
+        _written((grad_y,))
+    if need_weights and not fresh_weights:
+        _written((grad_weights,))
     return grad_y if need_y else None, grad_weights if need_weights else None
 
 
@@ -338,11 +369,16 @@ def matvec_w4(x, codes, scales, *, zeros=None, plan: Optional[ExpertPlan] = None
     zp = None if zeros is None else _packed("zeros", zeros, torch.uint8, (*lead, N, G), index)
     xp, xs = _matrix("x", x, plan.num_tokens if by_token else rows, K, x.dtype, index)
     columns = N // 2 if gated else N
-    if out is None:
+    fresh = out is None
+    if fresh:
         out = torch.empty((rows, columns), dtype=x.dtype, device=x.device)
+    else:
+        _result("out", out)
     op, os = _matrix("out", out, rows, columns, x.dtype, index)
     _call(_lib.load().moe_fp8_b200_matvec_w4, index, xp, xs, int(by_token), C.byref(_lib.W4(cp, sp, zp, E, N, K, K // G)),
           int(gated), op, os, kind, None if plan is None else plan._c, rows)
+    if not fresh:
+        _written((out,))
     return out
 
 

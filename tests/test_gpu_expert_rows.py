@@ -480,3 +480,40 @@ def test_numbers_that_pass_their_bits(pkg):
                  lambda: pkg.dispatch_backward(wide, plan), lambda: pkg.combine(wide, torch.rand(4, 2, device="cuda"), plan)):
         with pytest.raises(ValueError, match="columns"):
             call()
+
+
+def test_given_results_and_autograd(pkg):
+    """A tensor that a backward pass keeps, written again as a result, is noticed; results with a gradient are refused."""
+    T, K, E, H, cols = 6, 2, 8, 16, 64
+    ids = some_ids(T, K, E, 3)
+    plan = pkg.sort_tokens(ids, E)
+    x, w = torch.randn(T, H, device="cuda"), torch.rand(T, K, device="cuda")
+    y, dw = torch.randn(T * K, H, device="cuda"), torch.empty(T, K, device="cuda")
+    ones = torch.ones(T, H, device="cuda", requires_grad=True)
+    half = torch.randn(T * K, cols, device="cuda").bfloat16()
+    codes, scales = torch.zeros(16, cols // 2, dtype=torch.uint8, device="cuda"), torch.ones(16, 2, device="cuda").bfloat16()
+    out, rows = torch.empty(T, H, device="cuda"), torch.empty(T * K, H, device="cuda")
+    narrow = torch.empty(T * K, 16, device="cuda").bfloat16()
+    for given, call in ((rows, lambda t: pkg.dispatch(x, plan, rows=t)), (rows, lambda t: pkg.sort_and_dispatch(x, ids, E, rows=t)),
+                        (out, lambda t: pkg.combine(y, w, plan, out=t)), (out, lambda t: pkg.dispatch_backward(y, plan, out=t)),
+                        (rows, lambda t: pkg.combine_backward(x, y, w, plan, grad_y=t)),
+                        (dw, lambda t: pkg.combine_backward(x, y, w, plan, grad_weights=t)),
+                        (narrow, lambda t: pkg.matvec_w4(half, codes, scales, out=t))):
+        factor = torch.ones_like(given, requires_grad=True)
+        given.zero_()
+        loss = (factor * given).float().sum()
+        call(given)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            loss.backward()
+        leaf = given.clone().requires_grad_()
+        with pytest.raises(ValueError, match="requires a gradient"):
+            call(leaf)
+        with torch.no_grad():
+            call(leaf)
+        with torch.inference_mode():
+            call(torch.empty_like(given))
+    # a leaf of the forward pass next to given rows: refused before the plan is filled
+    filled = plan._filled
+    with pytest.raises(ValueError, match="rows cannot be given"):
+        pkg.sort_and_dispatch(ones, ids, E, plan=plan, rows=rows)
+    assert plan._filled == filled
