@@ -97,6 +97,8 @@ def _matrix(name, t, rows, columns, dtype, index):
 
 
 def _row_type(name, t):
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor")
     if t.dtype not in _ROW_TYPES:
         raise TypeError(f"{name} must be bfloat16, float16 or float32, got {t.dtype}")
     if t.dim() != 2 or not 1 <= t.shape[1] <= _MAX_COLUMNS:
@@ -228,6 +230,8 @@ def dispatch(x, plan: ExpertPlan, rows=None):
     a new matrix: zeros).  x [T, hidden], rows [plan.capacity, hidden]: bfloat16, float16 or float32, any row stride.
     Differentiable in x (not together with `rows`)."""
     _check_plan(plan)
+    if not isinstance(x, torch.Tensor):
+        raise TypeError("x must be a torch.Tensor")
     if _wants_grad(x):
         if rows is not None:
             raise ValueError("rows cannot be given where x requires a gradient")
@@ -242,6 +246,8 @@ def dispatch(x, plan: ExpertPlan, rows=None):
 def sort_and_dispatch(x, topk_idx, num_experts: int, *, first_expert: int = 0, align: int = 1,
                       plan: Optional[ExpertPlan] = None, rows=None) -> Tuple[torch.Tensor, ExpertPlan]:
     """sort_tokens and dispatch in one call: (rows, plan)."""
+    if not isinstance(x, torch.Tensor):
+        raise TypeError("x must be a torch.Tensor")
     plan = _ids(topk_idx, num_experts, first_expert, align, plan)
     if _wants_grad(x):
         if rows is not None:
@@ -278,6 +284,8 @@ def combine(y, weights, plan: ExpertPlan, out=None):
     without rows.  y [plan.capacity, hidden], weights fp32 [T, top_k].  Padding and unused rows of y are not read.
     Differentiable in y and weights (not together with `out`)."""
     _check_plan(plan)
+    if not isinstance(y, torch.Tensor) or not isinstance(weights, torch.Tensor):
+        raise TypeError("y and weights must be torch.Tensors")
     if _wants_grad(y, weights):
         if out is not None:
             raise ValueError("out cannot be given where y or weights require a gradient")

@@ -517,3 +517,18 @@ def test_given_results_and_autograd(pkg):
     with pytest.raises(ValueError, match="rows cannot be given"):
         pkg.sort_and_dispatch(ones, ids, E, plan=plan, rows=rows)
     assert plan._filled == filled
+
+
+def test_what_is_no_tensor(pkg):
+    ids = some_ids(4, 2, 8, 1)
+    plan = pkg.sort_tokens(ids, 8)
+    y, w = torch.randn(8, 16, device="cuda"), torch.rand(4, 2, device="cuda")
+    filled = plan._filled
+    for call in (lambda: pkg.combine(y, None, plan), lambda: pkg.combine(y.clone().requires_grad_(), None, plan),
+                 lambda: pkg.combine(None, w, plan), lambda: pkg.dispatch([[1.0]], plan), lambda: pkg.dispatch_backward(None, plan),
+                 lambda: pkg.sort_and_dispatch(None, ids, 8, plan=plan), lambda: pkg.combine_backward(None, y, w, plan),
+                 lambda: pkg.combine_backward(y[:4], y, None, plan), lambda: pkg.combine_backward(y[:4], None, w, plan),
+                 lambda: pkg.combine(y, w, plan, out=3)):
+        with pytest.raises(TypeError):
+            call()
+    assert plan._filled == filled
