@@ -721,7 +721,9 @@ cudaError_t launch_sort(const void* ids, int64_t first, const PlanView& p, cudaS
     const int threads = need >= kSortThreads ? kSortThreads : need <= 128 ? 128 : (need + 31) / 32 * 32;
     const size_t smem = sort_smem_bytes(threads, p.E);
     if (smem > 48 * 1024) {
-        const cudaError_t e = cudaFuncSetAttribute(sort_tokens_kernel<Id>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+        // the same value in every call: the attribute belongs to the kernel, and another thread's call may stand between this and the launch
+        const cudaError_t e = cudaFuncSetAttribute(sort_tokens_kernel<Id>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                   (int)sort_smem_bytes(kSortThreads, kMaxExperts));
         if (e != cudaSuccess) return e;
     }
     return launch_after(sort_tokens_kernel<Id>, dim3(ctas), dim3(threads), smem, ctas, stream, static_cast<const Id*>(ids),

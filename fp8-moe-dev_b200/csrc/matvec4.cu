@@ -120,6 +120,8 @@ struct Shared {
     alignas(16) float part[2][kWarps][128];
 };
 
+constexpr size_t kDynamicLimit = kSharedLimit - sizeof(Shared) - 256;
+
 // What the CTAs know of the experts' rows, behind the ring: [E + 1] each.
 struct Experts {
     int* first;    // tiles of x rows in front of expert e
@@ -847,7 +849,8 @@ cudaError_t launch_form(const MatvecArgs& a, const MatvecMaps& maps, int sms, cu
 {
     const size_t smem = (size_t)a.stages * a.stage_bytes + experts_bytes(a.E) + kSwizzleAtom;
     const auto kernel = matvec4_kernel<T, FINE, ZEROS, SPLIT>;
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    // the same value in every call: the attribute belongs to the kernel, and another thread's call may stand between this and the launch
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kDynamicLimit);
     if (e != cudaSuccess) return e;
     return launch_after(kernel, dim3(sms), dim3(kThreads), smem, 1, stream, a, maps);
 }
@@ -985,7 +988,7 @@ extern "C" int moe_fp8_b200_matvec_w4(const void* x, int64_t x_stride, int by_to
     a.scale_at = per_stage * a.chunks * 2048;
     a.zero_at = (a.scale_at + per_stage * kTileRows * a.scale_bytes + 127) / 128 * 128;
     a.stage_bytes = (a.zero_at + (w->zeros ? per_stage * kTileRows * a.zero_bytes : 0) + 1023) / 1024 * 1024;
-    a.stages = (int)((kSharedLimit - sizeof(Shared) - experts_bytes(a.E) - kSwizzleAtom - 256) / a.stage_bytes);
+    a.stages = (int)((kDynamicLimit - experts_bytes(a.E) - kSwizzleAtom) / a.stage_bytes);
     if (a.stages > kMaxStages) a.stages = kMaxStages;
     a.tile_bytes = kTileRows * (unsigned)(a.chunks * 128 + a.scale_bytes + (w->zeros ? a.zero_bytes : 0));
     MatvecMaps maps = {};

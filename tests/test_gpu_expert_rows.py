@@ -532,3 +532,43 @@ def test_what_is_no_tensor(pkg):
         with pytest.raises(TypeError):
             call()
     assert plan._filled == filled
+
+
+def calls_of_threads(pkg, make, sizes, rounds=6000, threads_per_size=3):
+    """Errors of C calls that several threads make at once, each with a stream and tensors of its own.  make(size): the entry point,
+    its arguments, and a check of the results."""
+    import ctypes as C
+    import threading
+    failed, start = [], threading.Barrier(len(sizes) * threads_per_size)
+
+    def calls(size):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                fn, args, check = make(size)
+                stream, err = torch.cuda.current_stream().cuda_stream, C.create_string_buffer(256)
+                torch.cuda.synchronize()
+                start.wait()
+                failed.extend(err.value for _ in range(rounds) if fn(*args, stream, err, 256) != pkg._lib.OK)
+                check()
+        except BaseException as e:
+            failed.append(e)
+            start.abort()
+
+    threads = [threading.Thread(target=calls, args=(size,)) for size in sizes for _ in range(threads_per_size)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    return failed
+
+
+def test_sorts_of_several_threads(pkg):
+    """Calls that need different amounts of shared memory of one kernel: what one sets for its launch holds for the other's."""
+    T, K = 400, 8
+
+    def make(E):
+        ids = some_ids(T, K, E, E)
+        plan = fresh_plan(pkg, T, K, E, 1)
+        return (pkg._lib.load().moe_fp8_b200_sort_tokens, (ids.data_ptr(), 32, 0, plan._c), lambda: check_plan(pkg, plan, ids, E, 0, 1))
+
+    assert not calls_of_threads(pkg, make, (1024, 400))

@@ -336,3 +336,23 @@ def test_sizes_beyond_32_bits(pkg):
     with pytest.raises(ValueError, match="too many"):
         pkg.matvec_w4(x, torch.empty((1 << 32) + 16, 32, dtype=torch.uint8, device="meta"),
                       torch.empty((1 << 32) + 16, 2, dtype=torch.bfloat16, device="meta"))
+
+
+def test_products_of_several_threads(pkg):
+    """Calls that need different amounts of shared memory of one kernel: what one sets for its launch holds for the other's."""
+    import ctypes as C
+    from test_gpu_expert_rows import calls_of_threads
+    N = 64
+
+    def make(K):
+        codes, scales, _ = make_weights((), N, K, 128, torch.bfloat16, False, K)
+        x, out = torch.ones(1, K, dtype=torch.bfloat16, device="cuda"), torch.empty(1, N, dtype=torch.bfloat16, device="cuda")
+        w = pkg._lib.W4(codes.data_ptr(), scales.data_ptr(), None, 1, N, K, 128)
+
+        def check():
+            want, bound = expect(x, decoded(codes, scales, None), False)
+            assert close(out, want, bound, torch.bfloat16)
+
+        return (pkg._lib.load().moe_fp8_b200_matvec_w4, (x.data_ptr(), K, 0, C.byref(w), 0, out.data_ptr(), N, 0, None, 1), check)
+
+    assert not calls_of_threads(pkg, make, (2048, 256))
