@@ -111,7 +111,8 @@ def _result(name, t):
         raise ValueError(f"{name} requires a gradient: give a tensor that does not, or call under torch.no_grad()")
 
 
-# autograd learns that a given tensor was written: a backward pass that saved it raises instead of reading the new contents
+# autograd learns that a given tensor, or an array of a plan, was written: a backward pass that saved it raises instead of reading the
+# new contents
 _written = torch._C._increment_version
 
 
@@ -140,7 +141,7 @@ class ExpertPlan:
 
     Made by sort_tokens, or from four tensors of one's own (to be filled, or filled elsewhere)."""
     __slots__ = ("pair_row", "row_pair", "expert_offset", "expert_count", "align", "num_tokens", "top_k", "num_experts",
-                 "capacity", "device", "index", "_c", "_filled")
+                 "capacity", "device", "index", "_c", "_arrays")
 
     def __init__(self, pair_row, row_pair, expert_offset, expert_count, *, align: int = 1):
         index = _on_gpu("pair_row", pair_row)
@@ -152,7 +153,7 @@ class ExpertPlan:
         self.capacity = capacity = plan_rows(T, K, E, align)
         self.pair_row, self.row_pair, self.expert_offset, self.expert_count = pair_row, row_pair, expert_offset, expert_count
         self.device, self.index = pair_row.device, index
-        self._filled = 0   # how often it was filled: a backward pass wants the plan of its forward pass
+        self._arrays = (pair_row, row_pair, expert_offset, expert_count)
         i32 = torch.int32
         self._c = C.byref(_lib.Plan(T, K, E, align, _packed("pair_row", pair_row, i32, (T, K), index),
                                     _packed("row_pair", row_pair, i32, (capacity,), index),
@@ -166,6 +167,21 @@ class ExpertPlan:
             return torch.empty(shape, dtype=torch.int32, device=device)
         return cls(ints(num_tokens, top_k), ints(plan_rows(num_tokens, top_k, num_experts, align)), ints(num_experts + 1),
                    ints(num_experts), align=align)
+
+    @property
+    def _filled(self):
+        """The versions of the arrays that a backward pass reads: any write to them changes these, through whichever object it went."""
+        return self.pair_row._version, self.expert_offset._version, self.expert_count._version
+
+    def _for_backward(self):
+        """The plan that a backward pass keeps, and its state: this one, if the versions of its arrays say when they are written.  They
+        do not for pieces of a larger buffer, whose version moves with the other pieces too, nor for tensors of the inference
+        mode, which have none: then a plan with copies, which no one else knows."""
+        read = (self.pair_row, self.expert_offset, self.expert_count)
+        if all(t.untyped_storage().nbytes() == 4 * t.numel() and not t.is_inference() for t in read):
+            return self, self._filled
+        plan = ExpertPlan(self.pair_row.clone(), self.row_pair, self.expert_offset.clone(), self.expert_count.clone(), align=self.align)
+        return plan, plan._filled
 
 
 def _check_plan(plan):
@@ -201,9 +217,9 @@ def sort_tokens(topk_idx, num_experts: int, *, first_expert: int = 0, align: int
     """Sorts the (token, expert) pairs of topk_idx [T, top_k] (int32 or int64) by expert.  The plan's experts are
     [first_expert, first_expert + num_experts); pairs of other experts (an id of -1, another GPU's expert) have no row."""
     plan = _ids(topk_idx, num_experts, first_expert, align, plan)
-    plan._filled += 1
     _call(_lib.load().moe_fp8_b200_sort_tokens, plan.index, topk_idx.data_ptr(), _ID_BITS[topk_idx.dtype], first_expert,
           plan._c)
+    _written(plan._arrays)
     return plan
 
 
@@ -254,11 +270,9 @@ def sort_and_dispatch(x, topk_idx, num_experts: int, *, first_expert: int = 0, a
             raise ValueError("rows cannot be given where x requires a gradient")
         return dispatch(x, sort_tokens(topk_idx, num_experts, first_expert=first_expert, align=align, plan=plan)), plan
     rows, args = _rows_for(x, plan, rows)
-    plan._filled += 1
     _call(_lib.load().moe_fp8_b200_sort_and_dispatch, plan.index, topk_idx.data_ptr(), _ID_BITS[topk_idx.dtype], first_expert,
           *args)
-    if not args[-1]:
-        _written((rows,))
+    _written(plan._arrays if args[-1] else (rows, *plan._arrays))
     return rows, plan
 
 
@@ -404,7 +418,7 @@ def _same_plan(ctx):
 class _Dispatch(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, plan):
-        ctx.plan, ctx.filled = plan, plan._filled
+        ctx.plan, ctx.filled = plan._for_backward()
         return dispatch(x.detach(), plan)
 
     @staticmethod
@@ -416,7 +430,7 @@ class _Dispatch(torch.autograd.Function):
 class _Combine(torch.autograd.Function):
     @staticmethod
     def forward(ctx, y, weights, plan):
-        ctx.plan, ctx.filled = plan, plan._filled
+        ctx.plan, ctx.filled = plan._for_backward()
         ctx.save_for_backward(y, weights)
         return _combine(y.detach(), weights.detach(), plan, None)
 

@@ -572,3 +572,74 @@ def test_sorts_of_several_threads(pkg):
         return (pkg._lib.load().moe_fp8_b200_sort_tokens, (ids.data_ptr(), 32, 0, plan._c), lambda: check_plan(pkg, plan, ids, E, 0, 1))
 
     assert not calls_of_threads(pkg, make, (1024, 400))
+
+
+def test_a_plan_filled_through_another_object(pkg):
+    """Two plans over the same four tensors, and writes to the arrays themselves: the backward pass notices all of them."""
+    T, K, E, H = 8, 2, 4, 16
+
+    def forward(plan, which):
+        x = torch.randn(T, H, device="cuda", requires_grad=True)
+        if which == "dispatch":
+            return pkg.sort_and_dispatch(x, some_ids(T, K, E, 1), E, plan=plan)[0]
+        pkg.sort_tokens(some_ids(T, K, E, 1), E, plan=plan)
+        return pkg.combine(torch.randn(T * K, H, device="cuda", requires_grad=True), torch.rand(T, K, device="cuda"), plan)
+
+    for which in ("dispatch", "combine"):
+        plan = pkg.ExpertPlan.empty(T, K, E)
+        arrays = (plan.pair_row, plan.row_pair, plan.expert_offset, plan.expert_count)
+        other, ids = pkg.ExpertPlan(*arrays), some_ids(T, K, E, 2)
+        views = pkg.ExpertPlan(*(t.view(t.shape) for t in arrays))
+        x = torch.randn(T, H, device="cuda")
+        for refill in (lambda: pkg.sort_tokens(ids, E, plan=other), lambda: pkg.sort_and_dispatch(x, ids, E, plan=other),
+                       lambda: pkg.sort_and_dispatch(x, ids, E, plan=other, rows=torch.empty(T * K, H, device="cuda")),
+                       lambda: pkg.sort_tokens(ids, E, plan=views), lambda: plan.pair_row.fill_(-1)):
+            out = forward(plan, which)
+            refill()
+            with pytest.raises(RuntimeError, match="filled anew"):
+                out.sum().backward()
+        forward(plan, which).sum().backward()
+
+
+def test_a_callers_graph_learns_that_the_plan_was_filled(pkg):
+    """A node outside this package that kept one of the plan's arrays raises too."""
+    T, K, E, H = 8, 2, 4, 16
+    plan = pkg.ExpertPlan.empty(T, K, E)
+    y = torch.randn(T * K, H, device="cuda", requires_grad=True)
+    factor = torch.randn(E + 1, device="cuda", requires_grad=True)
+    for use in (lambda: y.index_select(0, plan.pair_row.view(-1)), lambda: y.index_select(0, plan.row_pair),
+                lambda: factor * plan.expert_offset, lambda: factor[:E] * plan.expert_count):
+        pkg.sort_tokens(some_ids(T, K, E, 1), E, plan=plan)
+        loss = use().sum()
+        pkg.sort_tokens(some_ids(T, K, E, 2), E, plan=plan)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            loss.backward()
+
+
+@pytest.mark.parametrize("kind", ["one buffer", "inference"])
+def test_plans_whose_versions_say_nothing(pkg, kind):
+    """Pieces of one buffer, which share its version, and tensors of the inference mode, which have none: a plan filled next to this
+    one is no obstacle, and this one's own refill changes no gradient."""
+    T, K, E, H = 9, 2, 5, 16
+    sizes = (T * K, T * K, E + 1, E)
+    if kind == "one buffer":
+        pieces = torch.empty(2 * sum(sizes), dtype=torch.int32, device="cuda").split(sizes + sizes)
+    else:
+        with torch.inference_mode():
+            pieces = [torch.empty(n, dtype=torch.int32, device="cuda") for n in sizes + sizes]
+    plans = [pkg.ExpertPlan(p[0].view(T, K), *p[1:]) for p in (pieces[:4], pieces[4:])]
+    seeds, xs, ys, ws, losses = (1, 2), [], [], [], []
+    up, upr = torch.randn(T, H, device="cuda"), torch.randn(T * K, H, device="cuda")
+    for plan, seed in zip(plans, seeds):
+        xs.append(torch.randn(T, H, device="cuda", requires_grad=True))
+        ys.append(torch.randn(T * K, H, device="cuda", requires_grad=True))
+        ws.append(torch.rand(T, K, device="cuda", requires_grad=True))
+        rows, _ = pkg.sort_and_dispatch(xs[-1], some_ids(T, K, E + 2, seed), E, first_expert=1, plan=plan)
+        losses.append((rows * upr).sum() + (pkg.combine(ys[-1], ws[-1], plan) * up).sum())
+    pkg.sort_tokens(some_ids(T, K, E + 2, 3), E, first_expert=1, plan=plans[1])
+    for i, seed in enumerate(seeds):
+        losses[i].backward()
+        plan = pkg.sort_tokens(some_ids(T, K, E + 2, seed), E, first_expert=1)
+        dy, dw = pkg.combine_backward(up, ys[i].detach(), ws[i].detach(), plan)
+        assert torch.equal(xs[i].grad, pkg.dispatch_backward(upr, plan))
+        assert torch.equal(ys[i].grad, dy) and torch.equal(ws[i].grad, dw)
