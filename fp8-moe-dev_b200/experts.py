@@ -17,6 +17,7 @@ inside the reference's layer are kernel/moe_fp8.cu:1064-1115 (permute) and :2254
 from __future__ import annotations
 
 import ctypes as C
+import operator
 import threading
 from typing import Optional, Tuple
 
@@ -139,9 +140,12 @@ class ExpertPlan:
       expert_offset  int32 [E + 1]       first row of each expert, and the end of the last one
       expert_count   int32 [E]           pairs of each expert
 
-    Made by sort_tokens, or from four tensors of one's own (to be filled, or filled elsewhere)."""
-    __slots__ = ("pair_row", "row_pair", "expert_offset", "expert_count", "align", "num_tokens", "top_k", "num_experts",
-                 "capacity", "device", "index", "_c", "_arrays")
+    Made by sort_tokens, or from four tensors of one's own (to be filled, or filled elsewhere).  All of these are read-only."""
+    # the C struct holds the same addresses and sizes
+    __slots__ = ("_pair_row", "_row_pair", "_expert_offset", "_expert_count", "_align", "_num_tokens", "_top_k", "_num_experts",
+                 "_capacity", "_device", "_index", "_c", "_arrays")
+    (pair_row, row_pair, expert_offset, expert_count, align, num_tokens, top_k, num_experts, capacity, device,
+     index) = (property(operator.attrgetter(name)) for name in __slots__[:11])
 
     def __init__(self, pair_row, row_pair, expert_offset, expert_count, *, align: int = 1):
         index = _on_gpu("pair_row", pair_row)
@@ -149,10 +153,10 @@ class ExpertPlan:
             raise ValueError(f"pair_row must have shape (tokens, top_k), got {tuple(pair_row.shape)}")
         T, K = pair_row.shape
         E = expert_count.shape[0] if isinstance(expert_count, torch.Tensor) and expert_count.dim() == 1 else 0
-        self.num_tokens, self.top_k, self.num_experts, self.align = T, K, E, align
-        self.capacity = capacity = plan_rows(T, K, E, align)
-        self.pair_row, self.row_pair, self.expert_offset, self.expert_count = pair_row, row_pair, expert_offset, expert_count
-        self.device, self.index = pair_row.device, index
+        self._num_tokens, self._top_k, self._num_experts, self._align = T, K, E, align
+        self._capacity = capacity = plan_rows(T, K, E, align)
+        self._pair_row, self._row_pair, self._expert_offset, self._expert_count = pair_row, row_pair, expert_offset, expert_count
+        self._device, self._index = pair_row.device, index
         self._arrays = (pair_row, row_pair, expert_offset, expert_count)
         i32 = torch.int32
         self._c = C.byref(_lib.Plan(T, K, E, align, _packed("pair_row", pair_row, i32, (T, K), index),
@@ -171,23 +175,24 @@ class ExpertPlan:
     @property
     def _filled(self):
         """The versions of the arrays that a backward pass reads: any write to them changes these, through whichever object it went."""
-        return self.pair_row._version, self.expert_offset._version, self.expert_count._version
+        return self._pair_row._version, self._expert_offset._version, self._expert_count._version
 
     def _for_backward(self):
         """The plan that a backward pass keeps, and its state: this one, if the versions of its arrays say when they are written.  They
         do not for pieces of a larger buffer, whose version moves with the other pieces too, nor for tensors of the inference
         mode, which have none: then a plan with copies, which no one else knows."""
-        read = (self.pair_row, self.expert_offset, self.expert_count)
+        read = (self._pair_row, self._expert_offset, self._expert_count)
         if all(t.untyped_storage().nbytes() == 4 * t.numel() and not t.is_inference() for t in read):
             return self, self._filled
-        plan = ExpertPlan(self.pair_row.clone(), self.row_pair, self.expert_offset.clone(), self.expert_count.clone(), align=self.align)
+        plan = ExpertPlan(self._pair_row.clone(), self._row_pair, self._expert_offset.clone(), self._expert_count.clone(),
+                          align=self._align)
         return plan, plan._filled
 
 
 def _check_plan(plan):
     if not isinstance(plan, ExpertPlan):
         raise TypeError("plan must be an ExpertPlan")
-    return plan.index
+    return plan._index
 
 
 def _ids(topk_idx, num_experts, first_expert, align, plan):
@@ -205,10 +210,10 @@ def _ids(topk_idx, num_experts, first_expert, align, plan):
     if plan is None:
         return ExpertPlan.empty(T, K, int(num_experts), int(align), topk_idx.device)
     if _check_plan(plan) != index:
-        raise ValueError(f"plan must live on {topk_idx.device}, got {plan.device}")
-    if (plan.num_tokens, plan.top_k, plan.num_experts, plan.align) != (T, K, num_experts, align):
-        raise ValueError(f"plan is for {plan.num_tokens} tokens, top_k {plan.top_k}, {plan.num_experts} experts, align {plan.align}; "
-                         f"the call has {T}, {K}, {num_experts}, {align}")
+        raise ValueError(f"plan must live on {topk_idx.device}, got {plan._device}")
+    if (plan._num_tokens, plan._top_k, plan._num_experts, plan._align) != (T, K, num_experts, align):
+        raise ValueError(f"plan is for {plan._num_tokens} tokens, top_k {plan._top_k}, {plan._num_experts} experts, align "
+                         f"{plan._align}; the call has {T}, {K}, {num_experts}, {align}")
     return plan
 
 
@@ -217,7 +222,7 @@ def sort_tokens(topk_idx, num_experts: int, *, first_expert: int = 0, align: int
     """Sorts the (token, expert) pairs of topk_idx [T, top_k] (int32 or int64) by expert.  The plan's experts are
     [first_expert, first_expert + num_experts); pairs of other experts (an id of -1, another GPU's expert) have no row."""
     plan = _ids(topk_idx, num_experts, first_expert, align, plan)
-    _call(_lib.load().moe_fp8_b200_sort_tokens, plan.index, topk_idx.data_ptr(), _ID_BITS[topk_idx.dtype], first_expert,
+    _call(_lib.load().moe_fp8_b200_sort_tokens, plan._index, topk_idx.data_ptr(), _ID_BITS[topk_idx.dtype], first_expert,
           plan._c)
     _written(plan._arrays)
     return plan
@@ -227,13 +232,13 @@ def _rows_for(x, plan, rows):
     """Arguments of the copy to packed rows: the matrix, and its C arguments."""
     kind = _row_type("x", x)
     H = x.shape[1]
-    xp, xs = _matrix("x", x, plan.num_tokens, H, x.dtype, plan.index)
+    xp, xs = _matrix("x", x, plan._num_tokens, H, x.dtype, plan._index)
     fresh = rows is None
     if fresh:
-        rows = torch.empty((plan.capacity, H), dtype=x.dtype, device=plan.device)
+        rows = torch.empty((plan._capacity, H), dtype=x.dtype, device=plan._device)
     else:
         _result("rows", rows)
-    rp, rs = _matrix("rows", rows, plan.capacity, H, x.dtype, plan.index)
+    rp, rs = _matrix("rows", rows, plan._capacity, H, x.dtype, plan._index)
     return rows, (xp, xs, rp, rs, kind, H, plan._c, int(fresh))
 
 
@@ -253,7 +258,7 @@ def dispatch(x, plan: ExpertPlan, rows=None):
             raise ValueError("rows cannot be given where x requires a gradient")
         return _Dispatch.apply(x, plan)
     rows, args = _rows_for(x, plan, rows)
-    _call(_lib.load().moe_fp8_b200_dispatch_rows, plan.index, *args)
+    _call(_lib.load().moe_fp8_b200_dispatch_rows, plan._index, *args)
     if not args[-1]:
         _written((rows,))
     return rows
@@ -270,7 +275,7 @@ def sort_and_dispatch(x, topk_idx, num_experts: int, *, first_expert: int = 0, a
             raise ValueError("rows cannot be given where x requires a gradient")
         return dispatch(x, sort_tokens(topk_idx, num_experts, first_expert=first_expert, align=align, plan=plan)), plan
     rows, args = _rows_for(x, plan, rows)
-    _call(_lib.load().moe_fp8_b200_sort_and_dispatch, plan.index, topk_idx.data_ptr(), _ID_BITS[topk_idx.dtype], first_expert,
+    _call(_lib.load().moe_fp8_b200_sort_and_dispatch, plan._index, topk_idx.data_ptr(), _ID_BITS[topk_idx.dtype], first_expert,
           *args)
     _written(plan._arrays if args[-1] else (rows, *plan._arrays))
     return rows, plan
@@ -279,15 +284,15 @@ def sort_and_dispatch(x, topk_idx, num_experts: int, *, first_expert: int = 0, a
 def _combine(y, weights, plan, out):
     kind = _row_type("y", y)
     H = y.shape[1]
-    yp, ys = _matrix("y", y, plan.capacity, H, y.dtype, plan.index)
-    wp = None if weights is None else _packed("weights", weights, torch.float32, (plan.num_tokens, plan.top_k), plan.index)
+    yp, ys = _matrix("y", y, plan._capacity, H, y.dtype, plan._index)
+    wp = None if weights is None else _packed("weights", weights, torch.float32, (plan._num_tokens, plan._top_k), plan._index)
     fresh = out is None
     if fresh:
-        out = torch.empty((plan.num_tokens, H), dtype=y.dtype, device=plan.device)
+        out = torch.empty((plan._num_tokens, H), dtype=y.dtype, device=plan._device)
     else:
         _result("out", out)
-    op, os = _matrix("out", out, plan.num_tokens, H, y.dtype, plan.index)
-    _call(_lib.load().moe_fp8_b200_combine_rows, plan.index, yp, ys, wp, op, os, kind, H, plan._c)
+    op, os = _matrix("out", out, plan._num_tokens, H, y.dtype, plan._index)
+    _call(_lib.load().moe_fp8_b200_combine_rows, plan._index, yp, ys, wp, op, os, kind, H, plan._c)
     if not fresh:
         _written((out,))
     return out
@@ -320,25 +325,25 @@ def combine_backward(grad_out, y, weights, plan: ExpertPlan, grad_y=None, grad_w
     not needed is None."""
     _check_plan(plan)
     kind = _row_type("grad_out", grad_out)
-    H, dtype, device, index = grad_out.shape[1], grad_out.dtype, plan.device, plan.index
-    gp, gs = _matrix("grad_out", grad_out, plan.num_tokens, H, dtype, index)
-    yp, ys = _matrix("y", y, plan.capacity, H, dtype, index)
-    wp = _packed("weights", weights, torch.float32, (plan.num_tokens, plan.top_k), index)
+    H, dtype, device, index = grad_out.shape[1], grad_out.dtype, plan._device, plan._index
+    gp, gs = _matrix("grad_out", grad_out, plan._num_tokens, H, dtype, index)
+    yp, ys = _matrix("y", y, plan._capacity, H, dtype, index)
+    wp = _packed("weights", weights, torch.float32, (plan._num_tokens, plan._top_k), index)
     dp, ds, dwp = None, 0, None
     fresh = grad_y is None
     if need_y:
         if fresh:
-            grad_y = torch.empty((plan.capacity, H), dtype=dtype, device=device)
+            grad_y = torch.empty((plan._capacity, H), dtype=dtype, device=device)
         else:
             _result("grad_y", grad_y)
-        dp, ds = _matrix("grad_y", grad_y, plan.capacity, H, dtype, index)
+        dp, ds = _matrix("grad_y", grad_y, plan._capacity, H, dtype, index)
     fresh_weights = grad_weights is None
     if need_weights:
         if fresh_weights:
-            grad_weights = torch.empty((plan.num_tokens, plan.top_k), dtype=torch.float32, device=device)
+            grad_weights = torch.empty((plan._num_tokens, plan._top_k), dtype=torch.float32, device=device)
         else:
             _result("grad_weights", grad_weights)
-        dwp = _packed("grad_weights", grad_weights, torch.float32, (plan.num_tokens, plan.top_k), index)
+        dwp = _packed("grad_weights", grad_weights, torch.float32, (plan._num_tokens, plan._top_k), index)
     _call(_lib.load().moe_fp8_b200_combine_rows_backward, index, gp, gs, yp, ys, wp, dp, ds, dwp, kind, H, plan._c,
           int(fresh))
     if need_y and not fresh:
@@ -370,11 +375,11 @@ def matvec_w4(x, codes, scales, *, zeros=None, plan: Optional[ExpertPlan] = None
     if _wants_grad(x) or (isinstance(scales, torch.Tensor) and _wants_grad(scales)):
         raise ValueError("matvec_w4 has no gradient: call it under torch.no_grad()")
     if plan is not None and _check_plan(plan) != index:
-        raise ValueError(f"plan must live on {x.device}, got {plan.device}")
+        raise ValueError(f"plan must live on {x.device}, got {plan._device}")
     if by_token and plan is None:
         raise ValueError("by_token needs a plan")
     K = x.shape[1]
-    E = 1 if plan is None else plan.num_experts
+    E = 1 if plan is None else plan._num_experts
     if not isinstance(codes, torch.Tensor) or not isinstance(scales, torch.Tensor):
         raise TypeError("codes and scales must be torch.Tensors")
     lead = () if plan is None else (E,)
@@ -383,13 +388,13 @@ def matvec_w4(x, codes, scales, *, zeros=None, plan: Optional[ExpertPlan] = None
     N, G = codes.shape[-2], scales.shape[-1]
     if G < 1 or K % G or K % 2:
         raise ValueError(f"scales of {G} groups do not divide {K} columns")
-    rows = x.shape[0] if plan is None else plan.capacity
+    rows = x.shape[0] if plan is None else plan._capacity
     if rows >= 1 << 31 or N >= 1 << 31:
         raise ValueError(f"{rows} rows by {N} are too many")
     cp = _packed("codes", codes, torch.uint8, (*lead, N, K // 2), index)
     sp = _packed("scales", scales, x.dtype, (*lead, N, G), index)
     zp = None if zeros is None else _packed("zeros", zeros, torch.uint8, (*lead, N, G), index)
-    xp, xs = _matrix("x", x, plan.num_tokens if by_token else rows, K, x.dtype, index)
+    xp, xs = _matrix("x", x, plan._num_tokens if by_token else rows, K, x.dtype, index)
     columns = N // 2 if gated else N
     fresh = out is None
     if fresh:

@@ -643,3 +643,12 @@ def test_plans_whose_versions_say_nothing(pkg, kind):
         dy, dw = pkg.combine_backward(up, ys[i].detach(), ws[i].detach(), plan)
         assert torch.equal(xs[i].grad, pkg.dispatch_backward(upr, plan))
         assert torch.equal(ys[i].grad, dy) and torch.equal(ws[i].grad, dw)
+
+
+def test_a_plan_is_read_only(pkg):
+    plan = pkg.sort_tokens(some_ids(6, 2, 8, 4), 8)
+    for name in ("pair_row", "row_pair", "expert_offset", "expert_count", "align", "num_tokens", "top_k", "num_experts", "capacity",
+                 "device", "index"):
+        value = getattr(plan, name)
+        with pytest.raises(AttributeError):
+            setattr(plan, name, value)
