@@ -30,6 +30,7 @@ _ROW_TYPES = {torch.bfloat16: _lib.BF16, torch.float16: _lib.FP16, torch.float32
 _ID_BITS = {torch.int32: 32, torch.int64: 64}
 _raw_stream = torch._C._cuda_getCurrentRawStream
 _current_device = torch._C._cuda_getDevice
+_forward_ad = torch.autograd.forward_ad
 _MAX_COLUMNS = 1 << 24
 _SMALL = 1 << 20   # tokens up to which a plan's size needs no word from the library
 
@@ -107,7 +108,16 @@ def _row_type(name, t):
     return _ROW_TYPES[t.dtype]
 
 
+# Tangents of forward-mode differentiation go with tensors that want no gradient.  A result without one would say that it is zero.
+def _no_tangents(**tensors):
+    for name, t in tensors.items():
+        if isinstance(t, torch.Tensor) and _forward_ad.unpack_dual(t).tangent is not None:
+            raise NotImplementedError(f"{name} has a tangent, and there is no derivative in forward mode here")
+
+
 def _result(name, t):
+    if _forward_ad._current_level >= 0:
+        _no_tangents(**{name: t})
     if isinstance(t, torch.Tensor) and _wants_grad(t):
         raise ValueError(f"{name} requires a gradient: give a tensor that does not, or call under torch.no_grad()")
 
@@ -253,6 +263,8 @@ def dispatch(x, plan: ExpertPlan, rows=None):
     _check_plan(plan)
     if not isinstance(x, torch.Tensor):
         raise TypeError("x must be a torch.Tensor")
+    if _forward_ad._current_level >= 0:
+        _no_tangents(x=x)
     if _wants_grad(x):
         if rows is not None:
             raise ValueError("rows cannot be given where x requires a gradient")
@@ -269,6 +281,8 @@ def sort_and_dispatch(x, topk_idx, num_experts: int, *, first_expert: int = 0, a
     """sort_tokens and dispatch in one call: (rows, plan)."""
     if not isinstance(x, torch.Tensor):
         raise TypeError("x must be a torch.Tensor")
+    if _forward_ad._current_level >= 0:
+        _no_tangents(x=x)
     plan = _ids(topk_idx, num_experts, first_expert, align, plan)
     if _wants_grad(x):
         if rows is not None:
@@ -305,6 +319,8 @@ def combine(y, weights, plan: ExpertPlan, out=None):
     _check_plan(plan)
     if not isinstance(y, torch.Tensor) or not isinstance(weights, torch.Tensor):
         raise TypeError("y and weights must be torch.Tensors")
+    if _forward_ad._current_level >= 0:
+        _no_tangents(y=y, weights=weights)
     if _wants_grad(y, weights):
         if out is not None:
             raise ValueError("out cannot be given where y or weights require a gradient")
@@ -315,6 +331,8 @@ def combine(y, weights, plan: ExpertPlan, out=None):
 def dispatch_backward(grad_rows, plan: ExpertPlan, out=None):
     """Gradient of dispatch's x from that of its rows: out[t] = the sum of token t's rows."""
     _check_plan(plan)
+    if _forward_ad._current_level >= 0:
+        _no_tangents(grad_rows=grad_rows)
     return _combine(grad_rows, None, plan, out)
 
 
@@ -324,6 +342,8 @@ def combine_backward(grad_out, y, weights, plan: ExpertPlan, grad_y=None, grad_w
     experts' padding and untouched behind the last expert (in a new matrix: zero there too); grad_weights is 0 where a pair has no row.  A gradient that is
     not needed is None."""
     _check_plan(plan)
+    if _forward_ad._current_level >= 0:
+        _no_tangents(grad_out=grad_out, y=y, weights=weights)
     kind = _row_type("grad_out", grad_out)
     H, dtype, device, index = grad_out.shape[1], grad_out.dtype, plan._device, plan._index
     gp, gs = _matrix("grad_out", grad_out, plan._num_tokens, H, dtype, index)
@@ -372,6 +392,8 @@ def matvec_w4(x, codes, scales, *, zeros=None, plan: Optional[ExpertPlan] = None
     kind = _row_type("x", x)
     if kind == _lib.FP32:
         raise TypeError("x must be bfloat16 or float16, got torch.float32")
+    if _forward_ad._current_level >= 0:
+        _no_tangents(x=x, scales=scales)
     if _wants_grad(x) or (isinstance(scales, torch.Tensor) and _wants_grad(scales)):
         raise ValueError("matvec_w4 has no gradient: call it under torch.no_grad()")
     if plan is not None and _check_plan(plan) != index:

@@ -652,3 +652,34 @@ def test_a_plan_is_read_only(pkg):
         value = getattr(plan, name)
         with pytest.raises(AttributeError):
             setattr(plan, name, value)
+
+
+def test_forward_mode_tangents_are_refused(pkg):
+    """What would come back without its tangent raises, as it does where the input wants a gradient too."""
+    import torch.autograd.forward_ad as fwd
+    T, K, E, H = 6, 2, 8, 16
+    ids = some_ids(T, K, E, 4)
+    plan = pkg.sort_tokens(ids, E)
+    x, w = torch.randn(T, H, device="cuda"), torch.rand(T, K, device="cuda")
+    y = torch.randn(T * K, H, device="cuda")
+    half = torch.randn(T, 64, device="cuda").bfloat16()
+    codes, scales = torch.zeros(16, 32, dtype=torch.uint8, device="cuda"), torch.ones(16, 2, device="cuda").bfloat16()
+    calls = (("x", x, lambda t: pkg.dispatch(t, plan)), ("x", x, lambda t: pkg.sort_and_dispatch(t, ids, E, plan=plan)),
+             ("y", y, lambda t: pkg.combine(t, w, plan)), ("weights", w, lambda t: pkg.combine(y, t, plan)),
+             ("grad_rows", y, lambda t: pkg.dispatch_backward(t, plan)),
+             ("grad_out", x, lambda t: pkg.combine_backward(t, y, w, plan)), ("y", y, lambda t: pkg.combine_backward(x, t, w, plan)),
+             ("weights", w, lambda t: pkg.combine_backward(x, y, t, plan)),
+             ("x", half, lambda t: pkg.matvec_w4(t, codes, scales)), ("scales", scales, lambda t: pkg.matvec_w4(half, codes, t)),
+             # given results would keep a tangent of what they held before
+             ("rows", y, lambda t: pkg.dispatch(x, plan, rows=t)), ("out", x.clone(), lambda t: pkg.combine(y, w, plan, out=t)),
+             ("grad_y", y.clone(), lambda t: pkg.combine_backward(x, y, w, plan, grad_y=t)))
+    filled = plan._filled
+    with fwd.dual_level():
+        for name, t, call in calls:
+            with pytest.raises(NotImplementedError, match=f"{name}.*forward mode"):
+                call(fwd.make_dual(t, torch.ones_like(t)))
+            assert plan._filled == filled
+            with pytest.raises(NotImplementedError):
+                call(fwd.make_dual(t.clone().requires_grad_(), torch.ones_like(t)))
+            call(t)   # no tangent: as ever
+            filled = plan._filled
