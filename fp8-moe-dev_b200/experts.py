@@ -329,10 +329,12 @@ def combine(y, weights, plan: ExpertPlan, out=None):
 
 
 def dispatch_backward(grad_rows, plan: ExpertPlan, out=None):
-    """Gradient of dispatch's x from that of its rows: out[t] = the sum of token t's rows."""
+    """Gradient of dispatch's x from that of its rows: out[t] = the sum of token t's rows.  Not differentiable itself."""
     _check_plan(plan)
     if _forward_ad._current_level >= 0:
         _no_tangents(grad_rows=grad_rows)
+    if isinstance(grad_rows, torch.Tensor) and _wants_grad(grad_rows):
+        raise ValueError("dispatch_backward has no gradient: call it under torch.no_grad()")
     return _combine(grad_rows, None, plan, out)
 
 
@@ -340,10 +342,13 @@ def combine_backward(grad_out, y, weights, plan: ExpertPlan, grad_y=None, grad_w
                      need_weights: bool = True):
     """Gradients of combine: (grad_y [plan.capacity, hidden], grad_weights fp32 [T, top_k]).  grad_y is zero in the
     experts' padding and untouched behind the last expert (in a new matrix: zero there too); grad_weights is 0 where a pair has no row.  A gradient that is
-    not needed is None."""
+    not needed is None.  Not differentiable itself."""
     _check_plan(plan)
     if _forward_ad._current_level >= 0:
         _no_tangents(grad_out=grad_out, y=y, weights=weights)
+    for t in (grad_out, y, weights):
+        if isinstance(t, torch.Tensor) and t.requires_grad and torch.is_grad_enabled():
+            raise ValueError("combine_backward has no gradient: call it under torch.no_grad()")
     kind = _row_type("grad_out", grad_out)
     H, dtype, device, index = grad_out.shape[1], grad_out.dtype, plan._device, plan._index
     gp, gs = _matrix("grad_out", grad_out, plan._num_tokens, H, dtype, index)

@@ -683,3 +683,18 @@ def test_forward_mode_tangents_are_refused(pkg):
                 call(fwd.make_dual(t.clone().requires_grad_(), torch.ones_like(t)))
             call(t)   # no tangent: as ever
             filled = plan._filled
+
+
+def test_gradient_calls_on_tensors_that_want_a_gradient(pkg):
+    """dispatch_backward and combine_backward have no gradient of their own: they refuse instead of leaving the graph."""
+    T, K, E, H = 6, 2, 8, 16
+    plan = pkg.sort_tokens(some_ids(T, K, E, 4), E)
+    x, w, y = torch.randn(T, H, device="cuda"), torch.rand(T, K, device="cuda"), torch.randn(T * K, H, device="cuda")
+    for t, call in ((y, lambda t: pkg.dispatch_backward(t, plan)), (x, lambda t: pkg.combine_backward(t, y, w, plan)),
+                    (y, lambda t: pkg.combine_backward(x, t, w, plan)), (w, lambda t: pkg.combine_backward(x, y, t, plan))):
+        leaf = t.clone().requires_grad_()
+        with pytest.raises(ValueError, match="has no gradient"):
+            call(leaf)
+        with torch.no_grad():
+            call(leaf)
+        call(t)
