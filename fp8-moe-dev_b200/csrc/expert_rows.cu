@@ -510,7 +510,7 @@ __global__ void __launch_bounds__(kGradThreads, 3) combine_grad_kernel(Rows grad
 #pragma unroll
         for (int k = 0; k < kRowsAtOnce; ++k) {
             row[k] = k < rows ? live_row[base + k] : 0;
-            w[k] = k < rows ? weights[(long long)t * p.K + live_k[base + k]] : 0.0f;
+            w[k] = k < rows && grad_y.base ? weights[(long long)t * p.K + live_k[base + k]] : 0.0f;
             sum[k] = 0.0f;
         }
         for (int i = threadIdx.x; i < pieces; i += blockDim.x) {
@@ -902,7 +902,7 @@ int moe_fp8_b200_combine_rows_backward(const void* grad_out, int64_t grad_out_st
     int rc = check_plan(call, plan, p);
     if (rc != MOE_FP8_B200_OK || p.T == 0 || (!grad_y && !grad_weights)) return rc;
     rc = check_rows(call, "grad_out", grad_out, grad_out_stride, p.T, dtype, hidden, false, eg);
-    if (rc == MOE_FP8_B200_OK) rc = call.tensor("weights", weights, 4);
+    if (rc == MOE_FP8_B200_OK && (grad_y || weights)) rc = call.tensor("weights", weights, 4);
     if (rc == MOE_FP8_B200_OK && grad_y) {
         rc = check_rows(call, "grad_y", grad_y, grad_y_stride, p.capacity, dtype, hidden, true, ed);
         if (rc == MOE_FP8_B200_OK) rc = check_apart(call, ed, eg);

@@ -342,7 +342,8 @@ def combine_backward(grad_out, y, weights, plan: ExpertPlan, grad_y=None, grad_w
                      need_weights: bool = True):
     """Gradients of combine: (grad_y [plan.capacity, hidden], grad_weights fp32 [T, top_k]).  grad_y is zero in the
     experts' padding and untouched behind the last expert (in a new matrix: zero there too); grad_weights is 0 where a pair has no row.  A gradient that is
-    not needed is None.  Not differentiable itself."""
+    not needed is None; y is read for grad_weights only, weights for grad_y only, and either may be None without it.  Not
+    differentiable itself."""
     _check_plan(plan)
     if _forward_ad._current_level >= 0:
         _no_tangents(grad_out=grad_out, y=y, weights=weights)
@@ -352,9 +353,11 @@ def combine_backward(grad_out, y, weights, plan: ExpertPlan, grad_y=None, grad_w
     kind = _row_type("grad_out", grad_out)
     H, dtype, device, index = grad_out.shape[1], grad_out.dtype, plan._device, plan._index
     gp, gs = _matrix("grad_out", grad_out, plan._num_tokens, H, dtype, index)
-    yp, ys = _matrix("y", y, plan._capacity, H, dtype, index)
-    wp = _packed("weights", weights, torch.float32, (plan._num_tokens, plan._top_k), index)
-    dp, ds, dwp = None, 0, None
+    yp, ys, wp, dp, ds, dwp = None, 0, None, None, 0, None
+    if need_weights or y is not None:
+        yp, ys = _matrix("y", y, plan._capacity, H, dtype, index)
+    if need_y or weights is not None:
+        wp = _packed("weights", weights, torch.float32, (plan._num_tokens, plan._top_k), index)
     fresh = grad_y is None
     if need_y:
         if fresh:
@@ -463,7 +466,9 @@ class _Combine(torch.autograd.Function):
     @staticmethod
     def forward(ctx, y, weights, plan):
         ctx.plan, ctx.filled = plan._for_backward()
-        ctx.save_for_backward(y, weights)
+        # what neither gradient reads may be written, and freed, before the backward pass
+        need_y, need_weights, _ = ctx.needs_input_grad
+        ctx.save_for_backward(y if need_weights else None, weights if need_y else None)
         return _combine(y.detach(), weights.detach(), plan, None)
 
     @staticmethod

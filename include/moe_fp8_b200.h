@@ -482,8 +482,8 @@ MOE_FP8_B200_API int moe_fp8_b200_combine_rows(const void* y, int64_t y_stride, 
 
 /* The gradients of moe_fp8_b200_combine_rows: grad_y[r, :] = weights[pair] * grad_out[token, :] (padding rows zero,
  * unused rows left as they were, or zeroed too with zero_unused != 0) and grad_weights[t, k] = <grad_out[t, :], y[pair_row[t, k], :]>, summed in fp32 in a fixed
- * order (0 for a pair without a row).  Either may be NULL if it is not wanted; y is read for grad_weights only,
- * and may be NULL without it. */
+ * order (0 for a pair without a row).  Either may be NULL if it is not wanted; y is read for grad_weights only, weights
+ * for grad_y only, and either may be NULL without it. */
 MOE_FP8_B200_API int moe_fp8_b200_combine_rows_backward(const void* grad_out, int64_t grad_out_stride, const void* y,
                                                         int64_t y_stride, const float* weights, void* grad_y,
                                                         int64_t grad_y_stride, float* grad_weights, int dtype, int hidden,

@@ -698,3 +698,39 @@ def test_gradient_calls_on_tensors_that_want_a_gradient(pkg):
         with torch.no_grad():
             call(leaf)
         call(t)
+
+
+def test_combine_keeps_only_what_its_gradients_read(pkg):
+    """The gradient of y does not read y, that of the weights does not read the weights: either may be written after the pass."""
+    T, K, E, H = 7, 2, 4, 24
+    plan = pkg.sort_tokens(some_ids(T, K, E + 1, 5), E)
+    y0, w0, up = torch.randn(T * K, H, device="cuda"), torch.rand(T, K, device="cuda"), torch.randn(T, H, device="cuda")
+    dy, dw = pkg.combine_backward(up, y0, w0, plan)
+    leaf = y0.clone().requires_grad_()
+    y = leaf * 1.0
+    out = pkg.combine(y, w0, plan)
+    y.add_(1.0)
+    out.backward(up)
+    assert torch.equal(leaf.grad, dy)
+    leaf = w0.clone().requires_grad_()
+    w = leaf * 1.0
+    out = pkg.combine(y0, w, plan)
+    w.add_(1.0)
+    out.backward(up)
+    assert torch.equal(leaf.grad, dw)
+    # both wanted: both are read
+    for which in range(2):
+        y, w = y0.clone().requires_grad_() * 1.0, w0.clone().requires_grad_() * 1.0
+        out = pkg.combine(y, w, plan)
+        (y, w)[which].add_(1.0)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            out.backward(up)
+    # as plain calls
+    got, none = pkg.combine_backward(up, None, w0, plan, need_weights=False)
+    assert none is None and torch.equal(got, dy)
+    none, got = pkg.combine_backward(up, y0, None, plan, need_y=False)
+    assert none is None and torch.equal(got, dw)
+    for y, w, need_y, need_weights in ((None, w0, True, True), (None, w0, False, True), (y0, None, True, True), (y0, None, True, False)):
+        with pytest.raises(TypeError):
+            pkg.combine_backward(up, y, w, plan, need_y=need_y, need_weights=need_weights)
+    assert pkg.combine_backward(up, None, None, plan, need_y=False, need_weights=False) == (None, None)
