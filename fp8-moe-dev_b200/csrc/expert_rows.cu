@@ -800,9 +800,10 @@ cudaError_t launch_combine_grad(const Extent& grad_out, const Extent& y, const f
 }
 
 // The ids are read twice, by every CTA of the small kernel: the plan written over them would be read as ids.
-int check_ids(const Call& call, const void* ids, int id_bits, const PlanView& p)
+int check_ids(const Call& call, const void* ids, int id_bits, int64_t first, const PlanView& p)
 {
     if (id_bits != 32 && id_bits != 64) return call.bad("id_bits must be 32 or 64, got %d", id_bits);
+    if (first > INT64_MAX - (p.E - 1)) return call.bad("first_expert %lld: %d experts from it on are not 64-bit ids", (long long)first, p.E);
     const int rc = call.tensor("topk_idx", ids, id_bits / 8);
     return rc == MOE_FP8_B200_OK ? check_apart_from_plan(call, {"topk_idx", ids, 1, (int64_t)p.pairs * (id_bits / 8), 0}, p) : rc;
 }
@@ -825,7 +826,7 @@ int moe_fp8_b200_sort_tokens(const void* topk_idx, int id_bits, int64_t first_ex
     Call call{err, err_len};
     PlanView p;
     int rc = check_plan(call, plan, p);
-    if (rc == MOE_FP8_B200_OK && p.T > 0) rc = check_ids(call, topk_idx, id_bits, p);
+    if (rc == MOE_FP8_B200_OK && p.T > 0) rc = check_ids(call, topk_idx, id_bits, first_expert, p);
     if (rc != MOE_FP8_B200_OK) return rc;
     return call.cuda(enqueue_sort(topk_idx, id_bits, first_expert, p, static_cast<cudaStream_t>(stream)));
 }
@@ -854,7 +855,7 @@ int moe_fp8_b200_sort_and_dispatch(const void* topk_idx, int id_bits, int64_t fi
     PlanView p;
     Extent ex, er;
     int rc = check_plan(call, plan, p);
-    if (rc == MOE_FP8_B200_OK && p.T > 0) rc = check_ids(call, topk_idx, id_bits, p);
+    if (rc == MOE_FP8_B200_OK && p.T > 0) rc = check_ids(call, topk_idx, id_bits, first_expert, p);
     if (rc == MOE_FP8_B200_OK && p.T > 0) rc = check_rows(call, "x", x, x_stride, p.T, dtype, hidden, false, ex);
     if (rc == MOE_FP8_B200_OK && p.T > 0) rc = check_rows(call, "rows", rows, rows_stride, p.capacity, dtype, hidden, true, er);
     if (rc == MOE_FP8_B200_OK && p.T > 0) {

@@ -455,7 +455,7 @@ enum { MOE_FP8_B200_BF16 = 0, MOE_FP8_B200_FP16 = 1, MOE_FP8_B200_FP32 = 2 };
 MOE_FP8_B200_API int64_t moe_fp8_b200_plan_rows(int num_tokens, int top_k, int num_experts, int align);
 
 /* Fills the plan from expert ids [T, top_k] of id_bits = 32 or 64 bits each.  Any ids are safe; the same expert twice
- * in a token gives two rows. */
+ * in a token gives two rows.  The last expert, first_expert + num_experts - 1, has to be a 64-bit number too. */
 MOE_FP8_B200_API int moe_fp8_b200_sort_tokens(const void* topk_idx, int id_bits, int64_t first_expert,
                                               const moe_fp8_b200_plan* plan, void* stream, char* err, size_t err_len);
 

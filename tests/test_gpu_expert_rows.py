@@ -734,3 +734,23 @@ def test_combine_keeps_only_what_its_gradients_read(pkg):
         with pytest.raises(TypeError):
             pkg.combine_backward(up, y, w, plan, need_y=need_y, need_weights=need_weights)
     assert pkg.combine_backward(up, None, None, plan, need_y=False, need_weights=False) == (None, None)
+
+
+def test_first_experts_at_the_end_of_64_bits(pkg):
+    """An id is compared as a number: the experts behind the last 64-bit id are refused, they do not begin again at the first."""
+    lim = torch.iinfo(torch.int64)
+    ids = torch.tensor([[lim.min, lim.max], [lim.min + 2, lim.max - 2]], device="cuda")
+    x = torch.randn(2, 16, device="cuda")
+    for first, E in ((lim.max, 2), (lim.max - 2, 4)):
+        with pytest.raises(ValueError, match="64"):
+            pkg.sort_tokens(ids, E, first_expert=first)
+        with pytest.raises(ValueError, match="64"):
+            pkg.sort_and_dispatch(x, ids, E, first_expert=first)
+    for first, E in ((lim.max, 1), (lim.max - 3, 4), (lim.min, 4)):
+        check_plan(pkg, pkg.sort_tokens(ids, E, first_expert=first, plan=fresh_plan(pkg, 2, 2, E, 1)), ids, E, first, 1)
+    # the C entry by itself
+    import ctypes as C
+    lib, err = pkg._lib.load(), C.create_string_buffer(256)
+    plan = fresh_plan(pkg, 2, 2, 4, 1)
+    rc = lib.moe_fp8_b200_sort_tokens(ids.data_ptr(), 64, lim.max - 2, plan._c, None, err, 256)
+    assert rc == pkg._lib.ERR_INVALID_ARGUMENT and b"64-bit ids" in err.value
