@@ -208,7 +208,7 @@ def _check_plan(plan):
 def _ids(topk_idx, num_experts, first_expert, align, plan):
     """The plan to fill for these ids."""
     index = _on_gpu("topk_idx", topk_idx)
-    if not -1 << 63 <= first_expert <= (1 << 63) - max(1, num_experts):   # the library counts on from it modulo 2^64
+    if not -1 << 63 <= first_expert <= (1 << 63) - max(1, int(num_experts)):   # the library counts on from it modulo 2^64
         raise ValueError(f"first_expert {first_expert}: experts from it on are not 64-bit ids")
     if topk_idx.dtype not in _ID_BITS:
         raise TypeError(f"topk_idx must be int32 or int64, got {topk_idx.dtype}")

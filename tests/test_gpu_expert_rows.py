@@ -754,3 +754,12 @@ def test_first_experts_at_the_end_of_64_bits(pkg):
     plan = fresh_plan(pkg, 2, 2, 4, 1)
     rc = lib.moe_fp8_b200_sort_tokens(ids.data_ptr(), 64, lim.max - 2, plan._c, None, err, 256)
     assert rc == pkg._lib.ERR_INVALID_ARGUMENT and b"64-bit ids" in err.value
+
+
+def test_sizes_from_numpy(pkg):
+    ids = some_ids(4, 2, 8, 1)
+    want = pkg.sort_tokens(ids, 8, align=4)
+    got = pkg.sort_tokens(ids, np.int64(8), first_expert=np.int32(0), align=np.int64(4))
+    assert torch.equal(got.row_pair, want.row_pair)
+    got = pkg.sort_tokens(ids, np.int32(8), first_expert=np.int64(0), align=np.int32(4), plan=pkg.ExpertPlan.empty(4, 2, 8, 4))
+    assert torch.equal(got.row_pair, want.row_pair)
