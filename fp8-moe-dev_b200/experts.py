@@ -129,15 +129,16 @@ _written = torch._C._increment_version
 
 def plan_rows(num_tokens: int, top_k: int, num_experts: int, align: int = 1) -> int:
     """Rows that any choice of experts fits into: what `rows` of a dispatch must hold."""
-    T, K, E, align = int(num_tokens), int(top_k), int(num_experts), int(align)
-    if 0 <= T <= _SMALL and 1 <= K <= _lib.PLAN_MAX_TOP_K and 1 <= E <= _lib.PLAN_MAX_EXPERTS and 1 <= align <= 1024:
+    given = num_tokens, top_k, num_experts, align
+    T, K, E, align = whole = int(num_tokens), int(top_k), int(num_experts), int(align)
+    if whole == given and 0 <= T <= _SMALL and 1 <= K <= _lib.PLAN_MAX_TOP_K and 1 <= E <= _lib.PLAN_MAX_EXPERTS and 1 <= align <= 1024:
         pairs = T * K
         return (pairs + min(E, pairs) * (align - 1) + align - 1) // align * align
     # what passes 32 bits would reach the library cut to them
-    rows = _lib.load().moe_fp8_b200_plan_rows(T, K, E, align) if max(T, K, E, align) < 1 << 31 and min(T, K, E, align) >= 0 else -1
+    rows = _lib.load().moe_fp8_b200_plan_rows(*whole) if whole == given and max(whole) < 1 << 31 and min(whole) >= 0 else -1
     if rows < 0:
         raise ValueError(f"no plan for {num_tokens} tokens, top_k {top_k} (1 .. {_lib.PLAN_MAX_TOP_K}), {num_experts} experts "
-                         f"(1 .. {_lib.PLAN_MAX_EXPERTS}), align {align} (1 .. 1024)")
+                         f"(1 .. {_lib.PLAN_MAX_EXPERTS}), align {given[3]} (1 .. 1024)")
     return int(rows)
 
 
@@ -179,8 +180,9 @@ class ExpertPlan:
         """A plan to be filled."""
         def ints(*shape):
             return torch.empty(shape, dtype=torch.int32, device=device)
-        return cls(ints(num_tokens, top_k), ints(plan_rows(num_tokens, top_k, num_experts, align)), ints(num_experts + 1),
-                   ints(num_experts), align=align)
+        capacity = plan_rows(num_tokens, top_k, num_experts, align)
+        T, K, E = int(num_tokens), int(top_k), int(num_experts)
+        return cls(ints(T, K), ints(capacity), ints(E + 1), ints(E), align=int(align))
 
     @property
     def _filled(self):
@@ -208,6 +210,7 @@ def _check_plan(plan):
 def _ids(topk_idx, num_experts, first_expert, align, plan):
     """The plan to fill for these ids."""
     index = _on_gpu("topk_idx", topk_idx)
+    first_expert = operator.index(first_expert)
     if not -1 << 63 <= first_expert <= (1 << 63) - max(1, int(num_experts)):   # the library counts on from it modulo 2^64
         raise ValueError(f"first_expert {first_expert}: experts from it on are not 64-bit ids")
     if topk_idx.dtype not in _ID_BITS:
@@ -218,7 +221,7 @@ def _ids(topk_idx, num_experts, first_expert, align, plan):
         raise ValueError("topk_idx must be contiguous")
     T, K = topk_idx.shape
     if plan is None:
-        return ExpertPlan.empty(T, K, int(num_experts), int(align), topk_idx.device)
+        return ExpertPlan.empty(T, K, num_experts, align, topk_idx.device)
     if _check_plan(plan) != index:
         raise ValueError(f"plan must live on {topk_idx.device}, got {plan._device}")
     if (plan._num_tokens, plan._top_k, plan._num_experts, plan._align) != (T, K, num_experts, align):

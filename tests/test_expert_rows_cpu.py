@@ -89,3 +89,14 @@ def test_plan_sizes_beyond_32_bits(pkg, at, wrap):
     sizes[at] += wrap   # cut to 32 bits, a size that is allowed
     with pytest.raises(ValueError, match="no plan"):
         pkg.plan_rows(*sizes)
+
+
+@pytest.mark.parametrize("at", range(4))
+def test_plan_sizes_that_are_no_whole_numbers(pkg, at):
+    sizes = [5, 8, 16, 4]
+    rows = pkg.plan_rows(*sizes)
+    sizes[at] += 0.5
+    with pytest.raises(ValueError, match=f"no plan.*{sizes[at]}"):
+        pkg.plan_rows(*sizes)
+    sizes[at] -= 0.5   # the whole number, as a float
+    assert pkg.plan_rows(*sizes) == rows

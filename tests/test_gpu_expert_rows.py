@@ -763,3 +763,25 @@ def test_sizes_from_numpy(pkg):
     assert torch.equal(got.row_pair, want.row_pair)
     got = pkg.sort_tokens(ids, np.int32(8), first_expert=np.int64(0), align=np.int32(4), plan=pkg.ExpertPlan.empty(4, 2, 8, 4))
     assert torch.equal(got.row_pair, want.row_pair)
+
+
+def test_sizes_that_are_no_whole_numbers(pkg):
+    ids = some_ids(4, 2, 8, 1)
+    x = torch.randn(4, 16, device="cuda")
+    for wrong in (dict(num_experts=8.5), dict(num_experts=8, align=1.5)):
+        with pytest.raises(ValueError, match="no plan"):
+            pkg.sort_tokens(ids, **wrong)
+        with pytest.raises(ValueError, match="no plan"):
+            pkg.sort_and_dispatch(x, ids, **wrong)
+    plan = pkg.sort_tokens(ids, 8)
+    before = plan.pair_row.clone()
+    for call in (lambda: pkg.sort_tokens(ids + 1, 8, first_expert=0.5, plan=plan),
+                 lambda: pkg.sort_and_dispatch(x, ids + 1, 8, first_expert=0.5, plan=plan)):
+        with pytest.raises(TypeError):
+            call()
+    assert torch.equal(plan.pair_row, before)
+    with pytest.raises(ValueError, match="align 1.5"):
+        pkg.ExpertPlan.empty(4, 2, 8, 1.5)
+    same = pkg.sort_tokens(ids, np.int64(8), first_expert=np.int32(0), align=np.int64(1))
+    assert torch.equal(same.pair_row, before)
+    assert torch.equal(pkg.sort_tokens(ids, 8.0, align=1.0).pair_row, before)
