@@ -944,7 +944,9 @@ extern "C" int moe_fp8_b200_matvec_w4(const void* x, int64_t x_stride, int by_to
                              {"zeros", w->zeros, 1, all * groups, 0},
                              {"expert_offset", plan ? plan->expert_offset : nullptr, 1, 4ll * (w->num_experts + 1), 0},
                              {"expert_count", plan ? plan->expert_count : nullptr, 1, 4ll * w->num_experts, 0},
-                             {"row_pair", plan && by_token ? plan->row_pair : nullptr, 1, 4ll * rows, 0}};
+                             // not read here (row_pair without by_token), but what combines the results reads them
+                             {"pair_row", plan ? plan->pair_row : nullptr, 1, plan ? 4ll * plan->num_tokens * plan->top_k : 0, 0},
+                             {"row_pair", plan ? plan->row_pair : nullptr, 1, 4ll * rows, 0}};
     for (const Extent& in : inputs)
         if (share_memory(eo, in)) return bad("out and %s share memory", in.name);
 

@@ -356,3 +356,22 @@ def test_products_of_several_threads(pkg):
         return (pkg._lib.load().moe_fp8_b200_matvec_w4, (x.data_ptr(), K, 0, C.byref(w), 0, out.data_ptr(), N, 0, None, 1), check)
 
     assert not calls_of_threads(pkg, make, (2048, 256))
+
+
+@pytest.mark.parametrize("by_token", [False, True])
+def test_out_over_any_array_of_the_plan(pkg, by_token):
+    T, K, E, N, cols = 3, 2, 4, 16, 64
+    ids = torch.randint(0, E, (T, K), generator=torch.Generator().manual_seed(2)).int().cuda()
+    codes = torch.zeros(E, N, cols // 2, dtype=torch.uint8, device="cuda")
+    scales = torch.ones(E, N, 2, dtype=torch.bfloat16, device="cuda")
+    x = torch.ones(T if by_token else T * K, cols, dtype=torch.bfloat16, device="cuda")
+    shapes = dict(pair_row=(T, K), row_pair=(T * K,), expert_offset=(E + 1,), expert_count=(E,))
+    for field, shape in shapes.items():
+        memory = torch.zeros(T * K * N // 2, dtype=torch.int32, device="cuda")
+        arrays = {k: torch.empty(v, dtype=torch.int32, device="cuda") for k, v in shapes.items()}
+        arrays[field] = memory[:torch.Size(shape).numel()].view(shape)
+        plan = pkg.sort_tokens(ids, E, plan=pkg.ExpertPlan(**arrays))
+        kept = arrays[field].clone()
+        with pytest.raises(pkg.MoeError, match=f"out and {field} share memory"):
+            pkg.matvec_w4(x, codes, scales, plan=plan, by_token=by_token, out=memory.view(torch.bfloat16).view(T * K, N))
+        assert torch.equal(arrays[field], kept)
