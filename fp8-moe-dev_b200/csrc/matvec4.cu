@@ -20,7 +20,8 @@
 //   in the lower half and a second product takes the zero point off.  x is split, per row and warp, into four signed
 //   bytes of a 31-bit fixed-point number below the power of two above its largest value (exact for all values down to
 //   2^-23 of that, and off by 2^-31 of it below): four columns of the product per row, so two rows per instruction.
-//   The sums of a scale's products are exact integers, and become floats by starting from 1.5 * 2^23's bit pattern.
+//   The sums of a scale's products are exact integers, and become floats by starting from the bit pattern of 1.5 * 2^23 times a
+//   power of two, which brings them below 1/8, so that their products with any scales stay within fp32.
 // * More rows, or a row with an infinity or NaN, in the type itself (m16n8k16): 0x4300 | code is 128 + code in
 //   bf16 (0x6400 | code is 1024 + code in fp16), exactly, and so is the difference to 128 + zero.  11 (9) operations
 //   per eight codes instead of 3.
@@ -116,7 +117,7 @@ struct Shared {
     alignas(16) StageInfo info[kStageInfos];
     StageInfo start;                           // the first run's rows, before its weights are there
     unsigned begin, end;                       // this CTA's units
-    float unit[kWarps][kRowsOfX];              // a multiplying warp's scales of x's rows (see load_digits, load_values)
+    int unit[kWarps][kRowsOfX];                // of a multiplying warp's rows of x: a factor's bits (load_values) or a power (load_digits)
     alignas(16) float part[2][kWarps][128];
 };
 
@@ -270,12 +271,13 @@ __device__ __forceinline__ void mma_s8(int (&d)[4], const int (&c)[4], uint32_t 
 // The start of every sum by integers (see ByInteger).  With a scale per block there are so many that it is kept in four registers
 // (16 tokens, groups of 32 with zero points: 63 us, 67 with four moves per sum); with one per pair the registers are worth
 // more (one token, 256 experts: 39 us, 41 with Ones).
-constexpr int kOne = 0x4b400000;
+__host__ __device__ constexpr int one_of(bool zeros) { return 0x4b400000 - ((zeros ? 20 : 24) << 23); }
+template <bool ZEROS>
 struct Ones {
     int v[4];
     __device__ __forceinline__ Ones() {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) asm volatile("mov.b32 %0, %1;" : "=r"(v[i]) : "n"(kOne));
+        for (int i = 0; i < 4; ++i) asm volatile("mov.b32 %0, %1;" : "=r"(v[i]) : "n"(one_of(ZEROS)));
     }
 };
 // (a ^ b) & mask in one instruction
@@ -333,7 +335,7 @@ template <typename H, bool FINE, bool ZEROS, int SPLIT>
 struct ByType {
     static constexpr int kAtOnce = 1;
     template <int FIRST, int COUNT>
-    static __device__ __forceinline__ void multiply(float (&acc)[8], const uint32_t (&xr)[kMaxBlocks][4], const Ones& ones, const MatvecArgs& a, const TileView& v) {
+    static __device__ __forceinline__ void multiply(float (&acc)[8], const uint32_t (&xr)[kMaxBlocks][4], const Ones<ZEROS>& ones, const MatvecArgs& a, const TileView& v) {
         constexpr int kScales = FINE ? 2 : 1, kBlocks = 2 / kScales;   // scales of a pair, blocks of a scale
         const Words<SPLIT, COUNT> w(v, FIRST);
 #pragma unroll
@@ -361,18 +363,22 @@ struct ByType {
 };
 
 // By integers, for 2 * MMAS rows of x: column 4 r + d of a product is byte d of row r.  At most 64 products of 2^7 by 2^7 meet in
-// a sum, so it stays below 2^22 and kOne + sum is a float's bit pattern whose value is 1.5 * 2^23 + sum.
+// a sum (with zero points, of 15 by 2^7), so it stays below 2^22 and one_of + sum is a float's bit pattern whose value is
+// (1.5 * 2^23 + sum) / 2^24 (/ 2^20).  That makes the sum at most 1/16 (0.12), and the eight scales of a warp (sixteen of half as
+// many columns) add up to less than the largest of them: nothing leaves fp32 that the result does not leave.  At the other
+// end a product with a scale is rounded to 2^-149, half of which is 2^(e - 136) in the result, e as in load_digits.
 template <typename H, bool FINE, bool ZEROS, int SPLIT, int MMAS>
 struct ByInteger {
     static constexpr int kAtOnce = MMAS == 1 ? 2 : 1;
     template <int FIRST, int COUNT>
-    static __device__ __forceinline__ void multiply(float (&acc)[8], const uint32_t (&xr)[kMaxBlocks][4], const Ones& ones, const MatvecArgs& a, const TileView& v) {
+    static __device__ __forceinline__ void multiply(float (&acc)[8], const uint32_t (&xr)[kMaxBlocks][4], const Ones<ZEROS>& ones, const MatvecArgs& a, const TileView& v) {
         constexpr int kScales = FINE ? 2 : 1, kBlocks = 2 / kScales;
         const Words<SPLIT, COUNT> w(v, FIRST);
 #pragma unroll
         for (int p = 0; p < COUNT; ++p)
 #pragma unroll
             for (int i = 0; i < kScales; ++i) {
+                constexpr int kOne = one_of(ZEROS);
                 const Scales<H, ZEROS> s(a, v, FIRST + p, i != 0);
                 const uint32_t neg0 = __byte_perm(0u - s.z0, 0, 0), neg1 = __byte_perm(0u - s.z1, 0, 0);   // bytes -zero
                 int c[MMAS][4];
@@ -408,8 +414,8 @@ struct ByInteger {
 };
 
 // All of a warp's pairs, two at a time where the registers allow it.
-template <typename P, int FIRST = 0>
-__device__ __forceinline__ void multiply_pairs(float (&acc)[8], const uint32_t (&xr)[kMaxBlocks][4], const Ones& ones, const MatvecArgs& a, const TileView& v)
+template <typename P, int FIRST = 0, typename O>
+__device__ __forceinline__ void multiply_pairs(float (&acc)[8], const uint32_t (&xr)[kMaxBlocks][4], const O& ones, const MatvecArgs& a, const TileView& v)
 {
     if constexpr (2 * FIRST < kMaxBlocks) {
         if (v.blocks > 2 * (FIRST + P::kAtOnce - 1)) {
@@ -452,7 +458,7 @@ __device__ __forceinline__ int x_block(const MatvecArgs& a, int member, int j) {
 // (0, 4) (1, 5) (2, 6) (3, 7); zeros behind the last column.  A row of bf16 values near the end of fp32's range is held 2^16
 // times smaller, so that products with codes do not leave it; `unit` says so.
 template <typename T, int SPLIT>
-__device__ __forceinline__ void load_values(uint32_t (&xr)[kMaxBlocks][4], float* unit, const MatvecArgs& a, int row, int rows,
+__device__ __forceinline__ void load_values(uint32_t (&xr)[kMaxBlocks][4], int* unit, const MatvecArgs& a, int row, int rows,
                                             int member, int lane)
 {
     const int g = lane / 4, t = lane % 4;
@@ -500,17 +506,17 @@ __device__ __forceinline__ void load_values(uint32_t (&xr)[kMaxBlocks][4], float
             if (large) by_row = 65536.0f;
         }
     }
-    if (t == 0) unit[g] = by_row;
+    if (t == 0) unit[g] = __float_as_int(by_row);
     __syncwarp();
 }
 
 // x for the products by integers: thread (g, t) holds byte g % 4 of rows g / 4 and 2 + g / 4, of the columns 8t, 8t+2, 8t+4,
 // 8t+6 in one word and of the odd ones in the next.  A value is 31 bits below 2^e, the power of two above the largest of
 // its row's values in this warp, split into signed bytes.  Each thread converts two columns of a block; four threads'
-// words are then transposed byte by byte.  `unit` gets 2^(e - 1) of each row.  Returns the form that x is in (1 up to two rows, 2 up to four), or 0 if a value is not
+// words are then transposed byte by byte.  `unit` gets e of each row.  Returns the form that x is in (1 up to two rows, 2 up to four), or 0 if a value is not
 // finite.
 template <typename T, int SPLIT>
-__device__ __forceinline__ int load_digits(uint32_t (&xr)[kMaxBlocks][4], float* unit, const MatvecArgs& a, int row, int rows,
+__device__ __forceinline__ int load_digits(uint32_t (&xr)[kMaxBlocks][4], int* unit, const MatvecArgs& a, int row, int rows,
                                            int member, int lane)
 {
     const int t = lane % 4, q = lane / 4 % 4, forms = rows <= 2 ? 1 : 2;
@@ -540,7 +546,7 @@ __device__ __forceinline__ int load_digits(uint32_t (&xr)[kMaxBlocks][4], float*
         if (__any_sync(~0u, most >= Half2<T>::kInf)) return 0;
         const int e = (int)(most >> Half2<T>::kMantissa) - Half2<T>::kBias + 1;   // all below 2^e
         const float scale = exp2_of(-e);
-        if (lane % 16 == 0) unit[2 * m + lane / 16] = exp2_of(e - 1);
+        if (lane % 16 == 0) unit[2 * m + lane / 16] = e;
 #pragma unroll
         for (int j = 0; j < kMaxBlocks; ++j)
 #pragma unroll
@@ -762,10 +768,10 @@ __global__ void __launch_bounds__(kThreads, 1) matvec4_kernel(const MatvecArgs a
         const int pairs = ((a.K + 63) / 64 - member + SPLIT - 1) / SPLIT;
         view.blocks = pairs > 0 ? min(2 * pairs, a.K / 32 - 2 * (member + (pairs - 1) * SPLIT) + 2 * (pairs - 1)) : 0;
     }
-    const Ones ones;
+    const Ones<ZEROS> ones;
     uint32_t xr[kMaxBlocks][4];
     int form = 0;                      // 0 in the type itself, 1 by integers for up to two rows, 2 for up to four
-    float* const unit = sh.unit[warp];
+    int* const unit = sh.unit[warp];
     int slot = 0, lap = 0, row = -1;
     // round -1 only takes up the first x, while its weights are on their way
     for (int it = -1;; ++it) {
@@ -794,7 +800,7 @@ __global__ void __launch_bounds__(kThreads, 1) matvec4_kernel(const MatvecArgs a
             const int at = slot * a.stage_bytes;
             v.ring += at;
             if (form == 1) multiply_pairs<ByInteger<H, FINE, ZEROS, SPLIT, 1>>(acc, xr, ones, a, v);
-            else if (!ZEROS && form == 2) multiply_pairs<ByInteger<H, FINE, false, SPLIT, 2>>(acc, xr, ones, a, v);
+            else if (!ZEROS && form == 2) multiply_pairs<ByInteger<H, FINE, ZEROS, SPLIT, 2>>(acc, xr, ones, a, v);
             else multiply_pairs<ByType<H, FINE, ZEROS, SPLIT>>(acc, xr, ones, a, v);
         }
         __syncwarp();
@@ -804,15 +810,18 @@ __global__ void __launch_bounds__(kThreads, 1) matvec4_kernel(const MatvecArgs a
         float* part = sh.part[b][warp];
         if (form == 0) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) part[i * 32 + lane] = acc[i] * unit[2 * t + (i & 1)];
+            for (int i = 0; i < 4; ++i) part[i * 32 + lane] = acc[i] * __int_as_float(unit[2 * t + (i & 1)]);
         } else {
-            // this thread's columns 2t, 2t + 1 are bytes 0, 1 (t even) or 2, 3 of x row t / 2 (and 2 + t / 2)
-            const float low = (t & 1 ? 65536.0f : 1.0f) * (ZEROS ? 0x1p-29f : 0x1p-33f);
+            // this thread's columns 2t, 2t + 1 are bytes 0, 1 (t even) or 2, 3 of x row t / 2 (and 2 + t / 2).  With the larger one as
+            // the unit they stand for 2^(e - 2) and 2^(e + 14), which is multiplied in as two halves: neither leaves the range alone.
 #pragma unroll
             for (int m = 0; m < 2; ++m) {
                 if (m >= form) break;
-                float y0 = fmaf(256.0f, acc[4 * m + 1], acc[4 * m]) * low * unit[2 * m + (t >> 1)];
-                float y1 = fmaf(256.0f, acc[4 * m + 3], acc[4 * m + 2]) * low * unit[2 * m + (t >> 1)];
+                const int half = (unit[2 * m + (t >> 1)] >> 1) + 8 * (t & 1);
+                const int rest = unit[2 * m + (t >> 1)] + 16 * (t & 1) - half;
+                const float f0 = __int_as_float((half + 127) << 23), f1 = __int_as_float((rest + 125) << 23);
+                float y0 = fmaf(0x1p-8f, acc[4 * m], acc[4 * m + 1]) * f0 * f1;
+                float y1 = fmaf(0x1p-8f, acc[4 * m + 2], acc[4 * m + 3]) * f0 * f1;
                 y0 += __shfl_xor_sync(~0u, y0, 1);
                 y1 += __shfl_xor_sync(~0u, y1, 1);
                 part[((t & 1) * 2 + (t >> 1)) * 32 + g * 4 + m] = t & 1 ? y1 : y0;

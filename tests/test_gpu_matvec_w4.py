@@ -375,3 +375,23 @@ def test_out_over_any_array_of_the_plan(pkg, by_token):
         with pytest.raises(pkg.MoeError, match=f"out and {field} share memory"):
             pkg.matvec_w4(x, codes, scales, plan=plan, by_token=by_token, out=memory.view(torch.bfloat16).view(T * K, N))
         assert torch.equal(arrays[field], kept)
+
+
+@pytest.mark.parametrize("M", [1, 2, 3, 4, 6])
+@pytest.mark.parametrize("zeros", [False, True])
+@pytest.mark.parametrize("group", [32, 128])
+def test_scales_of_any_magnitude(pkg, M, zeros, group):
+    """bf16 scales near either end of fp32's range, with x that brings the results back into it.  A product with a scale is held
+    to half of fp32's smallest step, 2^-150; in front of it stands at most 2^14 times the power of two above the largest x, and at
+    most K / 32 products of each of four bytes, each byte worth 2^-8 of the next one, meet in a result."""
+    N, K = 64, 2048
+    for shift_x, shift_s in ((-60, 105), (-100, 125), (-125, 120), (0, 100), (0, -100), (60, -115), (100, -125), (118, -126)):
+        codes, scales, z = make_weights((), N, K, group, torch.bfloat16, zeros, M)
+        scales = (scales.double() * 2.0 ** shift_s).bfloat16()
+        x = torch.randn(M, K, generator=torch.Generator(device="cuda").manual_seed(M), device="cuda").double()
+        x = (x * 2.0 ** shift_x).bfloat16()
+        want, bound = expect(x, decoded(codes, scales, z), False)
+        assert bool(torch.isfinite(want.bfloat16()).all())
+        bound = bound + 1.01 * K / 32 * 2.0 ** -150 * 2.0 ** 14 * 2 * x.double().abs().amax(1, keepdim=True)
+        got = pkg.matvec_w4(x, codes, scales, zeros=z)
+        assert close(got, want, bound, torch.bfloat16), (shift_x, shift_s)
