@@ -18,15 +18,16 @@
 // * Up to four rows of x (two with zero points), by integers (m16n8k32, s8).  A code becomes a signed byte with a shift and a mask per four:
 //   (code - 8) * 16 sits in the upper half of a byte already, once its top bit is flipped; with zero points the code stays
 //   in the lower half and a second product takes the zero point off.  x is split, per row and warp, into four signed
-//   bytes of a 31-bit fixed-point number below the power of two above its largest value (exact for all values down to
-//   2^-23 of that, and off by 2^-31 of it below): four columns of the product per row, so two rows per instruction.
+//   bytes of a 31-bit fixed-point number below the power of two above its largest value: four columns of the product per row, so
+//   two rows per instruction.  Such a number is x itself for all values down to 2^-23 of that power (fp16: 2^-20); where a smaller
+//   one is not, the warp takes the other form, since it would be lost where a weight of zero meets the largest value.
 //   The sums of a scale's products are exact integers, and become floats by starting from the bit pattern of 1.5 * 2^23 times a
 //   power of two, which brings them below 1/8, so that their products with any scales stay within fp32.
-// * More rows, or a row with an infinity or NaN, in the type itself (m16n8k16): 0x4300 | code is 128 + code in
+// * More rows, or a row with an infinity, a NaN or values too far apart, in the type itself (m16n8k16): 0x4300 | code is 128 + code in
 //   bf16 (0x6400 | code is 1024 + code in fp16), exactly, and so is the difference to 128 + zero.  11 (9) operations
 //   per eight codes instead of 3.
 //
-// Either way the products are summed exactly or in fp32, scaled in fp32 per 32 or 64 columns, and rounded once.
+// Either way the products are exact and summed exactly or in fp32, scaled in fp32 per 32 or 64 columns, and rounded once.
 // The order of K inside a block of 32 columns is free as long as both operands agree: a thread's 32-bit word of codes
 // holds the columns 8t .. 8t+7 (t = lane % 4), and x is held in registers in the order they fall out of it.
 #include <cuda.h>
@@ -456,7 +457,8 @@ __device__ __forceinline__ int x_block(const MatvecArgs& a, int member, int j) {
 
 // x for the products in its own type: thread (g, t) holds row g's columns 8t .. 8t+7 of each of its warp's blocks, as the pairs
 // (0, 4) (1, 5) (2, 6) (3, 7); zeros behind the last column.  A row of bf16 values near the end of fp32's range is held 2^16
-// times smaller, so that products with codes do not leave it; `unit` says so.
+// times smaller, so that products with codes do not leave it; `unit` says so.  (Only values below 2^-110, 2^-222 of the largest one,
+// lose bits by that.)
 template <typename T, int SPLIT>
 __device__ __forceinline__ void load_values(uint32_t (&xr)[kMaxBlocks][4], int* unit, const MatvecArgs& a, int row, int rows,
                                             int member, int lane)
@@ -513,8 +515,8 @@ __device__ __forceinline__ void load_values(uint32_t (&xr)[kMaxBlocks][4], int* 
 // x for the products by integers: thread (g, t) holds byte g % 4 of rows g / 4 and 2 + g / 4, of the columns 8t, 8t+2, 8t+4,
 // 8t+6 in one word and of the odd ones in the next.  A value is 31 bits below 2^e, the power of two above the largest of
 // its row's values in this warp, split into signed bytes.  Each thread converts two columns of a block; four threads'
-// words are then transposed byte by byte.  `unit` gets e of each row.  Returns the form that x is in (1 up to two rows, 2 up to four), or 0 if a value is not
-// finite.
+// words are then transposed byte by byte.  `unit` gets e of each row.  Returns the form that
+// x is in (1 up to two rows, 2 up to four), or 0 if a value is not finite or has bits below 2^(e - 30).
 template <typename T, int SPLIT>
 __device__ __forceinline__ int load_digits(uint32_t (&xr)[kMaxBlocks][4], int* unit, const MatvecArgs& a, int row, int rows,
                                            int member, int lane)
@@ -525,7 +527,7 @@ __device__ __forceinline__ int load_digits(uint32_t (&xr)[kMaxBlocks][4], int* u
     for (int m = 0; m < 2; ++m) {
         if (m >= forms) break;
         const uint8_t* xp = x_row(a, row, rows, 2 * m + lane / 16, member) + 16 * t + 4 * q;
-        uint32_t raw[kMaxBlocks], most = 0;
+        uint32_t raw[kMaxBlocks], most = 0, least = ~0u;   // least: of the values but zero, minus one
         if (a.x_wide) {
 #pragma unroll
             for (int j = 0; j < kMaxBlocks; ++j) raw[j] = *reinterpret_cast<const uint32_t*>(xp + x_block<SPLIT>(a, member, j));
@@ -539,11 +541,16 @@ __device__ __forceinline__ int load_digits(uint32_t (&xr)[kMaxBlocks][4], int* u
 #pragma unroll
         for (int j = 0; j < kMaxBlocks; ++j) {
             if (!block_exists<SPLIT>(a, member, j)) raw[j] = 0;
-            most = max(most, max(raw[j] & 0x7fffu, raw[j] >> 16 & 0x7fffu));
+            const uint32_t lo = raw[j] & 0x7fffu, hi = raw[j] >> 16 & 0x7fffu;
+            most = max(most, max(lo, hi));
+            least = min(least, min(lo - 1, hi - 1));
         }
 #pragma unroll
         for (int d = 1; d < 16; d <<= 1) most = max(most, __shfl_xor_sync(~0u, most, d));
-        if (__any_sync(~0u, most >= Half2<T>::kInf)) return 0;
+        // the last bit of a value lies kMantissa below its first one; a subnormal's where the smallest normal one's does
+        const int lowest = (int)(most >> Half2<T>::kMantissa) - 29 + Half2<T>::kMantissa;
+        const uint32_t exact = lowest > 1 ? ((uint32_t)lowest << Half2<T>::kMantissa) - 1 : 0;
+        if (__any_sync(~0u, most >= Half2<T>::kInf || least < exact)) return 0;
         const int e = (int)(most >> Half2<T>::kMantissa) - Half2<T>::kBias + 1;   // all below 2^e
         const float scale = exp2_of(-e);
         if (lane % 16 == 0) unit[2 * m + lane / 16] = e;

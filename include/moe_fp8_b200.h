@@ -511,10 +511,12 @@ typedef struct moe_fp8_b200_w4 {
  * were.  Without a plan there is one matrix (num_experts 1) and x and out have num_rows rows.
  * gated: the weights are n / 2 linear rows followed by n / 2 gated ones, as in gemm1_weights of moe_fp8_b200_args, and out
  * [.., n / 2] is silu(y[r, n / 2 + i]) * y[r, i] (with zero points the number of groups is then even).
- * For decode batches (at most 2^21 rows): the weights are read once per eight rows of an expert.  Up to four rows of an
- * expert (two with zero points) go by exact integer products of x as 31-bit numbers below the power of two above the largest value of a row (in a
- * sixteenth to a quarter of its columns), which differ from x by at most 2^-31 of that power.  A load that never comes (a
- * second) leaves NaN.  No handle, as for the plan's functions. */
+ * For decode batches (at most 2^21 rows): the weights are read once per eight rows of an expert.  Every product of a code and
+ * an x is exact (but for bf16 values below 2^-110 in a row with one of 2^112 or more); what is rounded is their sum, in fp32, and
+ * its products with the scales, which are held to 2^-135 of the row's largest x at least.  The order of the sum depends on how
+ * many rows the expert has (up to four, two with zero points, or more) and on the values, so that a row's last bits may
+ * differ between batches; equal calls give equal bits.  A load that never comes (a second) leaves NaN and no error.  No
+ * handle, as for the plan's functions. */
 MOE_FP8_B200_API int moe_fp8_b200_matvec_w4(const void* x, int64_t x_stride, int by_token, const moe_fp8_b200_w4* w, int gated,
                                             void* out, int64_t out_stride, int dtype, const moe_fp8_b200_plan* plan,
                                             int num_rows, void* stream, char* err, size_t err_len);

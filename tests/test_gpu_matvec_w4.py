@@ -395,3 +395,45 @@ def test_scales_of_any_magnitude(pkg, M, zeros, group):
         bound = bound + 1.01 * K / 32 * 2.0 ** -150 * 2.0 ** 14 * 2 * x.double().abs().amax(1, keepdim=True)
         got = pkg.matvec_w4(x, codes, scales, zeros=z)
         assert close(got, want, bound, torch.bfloat16), (shift_x, shift_s)
+
+
+@pytest.mark.parametrize("M", [1, 2, 3, 4, 6])
+@pytest.mark.parametrize("zeros", [False, True])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_an_outlier_that_meets_no_weight(pkg, M, zeros, dtype):
+    """A large x whose weights are zero takes nothing away from the small ones: sums of exact products in fp32."""
+    N, K, group, at = 64, 2048, 128, 77
+    codes, scales, z = make_weights((), N, K, group, dtype, zeros, M)
+    codes[:32, at // 2] = codes[:32, at // 2] & 15 | ((z[:32, at // group] if zeros else 8) << 4)   # an odd column: the upper half
+    large, small = (2.0 ** 30, 2.0 ** -6) if dtype == torch.bfloat16 else (2.0 ** 15, 2.0 ** -17)
+    x = (torch.randn(M, K, generator=torch.Generator(device="cuda").manual_seed(M), device="cuda") * small).to(dtype)
+    x[0, at] = large
+    x[M - 1, at] = -large
+    w = decoded(codes, scales, z)
+    assert not w[:32, at].any() and bool(w[32:, at].any())
+    got = pkg.matvec_w4(x, codes, scales, zeros=z)
+    want, mag = x.double() @ w.t(), x.double().abs() @ w.abs().t()
+    # as in expect, without its term for an inexact x
+    assert close(got, want, (34 * 2.0 ** -23 + (2 * 16 + 16) * 2.0 ** -24) * mag, dtype)
+
+
+@pytest.mark.parametrize("M", [1, 2, 3, 4])
+@pytest.mark.parametrize("zeros", [False, True])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_a_small_value_under_a_large_one_is_exact(pkg, M, zeros, dtype):
+    """One column of weight one, the others zero: the result is that column of x, however far it lies below the largest value."""
+    N, K = 16, 64
+    mid = 5 if zeros else 8
+    codes = torch.full((N, K // 2), mid * 17, dtype=torch.uint8, device="cuda")
+    codes[:, 20] = mid + 1 | mid << 4   # column 40
+    z = torch.full((N, 1), mid, dtype=torch.uint8, device="cuda") if zeros else None
+    scales = torch.ones(N, 1, dtype=dtype, device="cuda")
+    info, top = torch.finfo(dtype), 2.0 ** (100 if dtype == torch.bfloat16 else 15)
+    for k in range(1, 42 if dtype == torch.bfloat16 else 39):
+        small = (1 + info.eps) * top * 2.0 ** -k   # all of its bits, fewer where fp16 is subnormal
+        x = torch.zeros(M, K, dtype=dtype, device="cuda")
+        x[:, 7], x[M - 1, 40] = -top, small
+        want = torch.zeros(M, N, dtype=dtype, device="cuda")
+        want[M - 1] = x[M - 1, 40]
+        assert bool(want[M - 1].any())
+        assert torch.equal(pkg.matvec_w4(x, codes, scales, zeros=z), want), k
