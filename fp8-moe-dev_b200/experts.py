@@ -32,7 +32,7 @@ _raw_stream = torch._C._cuda_getCurrentRawStream
 _current_device = torch._C._cuda_getDevice
 _forward_ad = torch.autograd.forward_ad
 _MAX_COLUMNS = 1 << 24
-_SMALL = 1 << 20   # tokens up to which a plan's size needs no word from the library
+_SMALL = 1 << 20   # tokens up to which a plan's size needs no word from the library, first experts that need no closer look
 
 
 class _Text(threading.local):
@@ -101,11 +101,12 @@ def _matrix(name, t, rows, columns, dtype, index):
 def _row_type(name, t):
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a torch.Tensor")
-    if t.dtype not in _ROW_TYPES:
+    kind = _ROW_TYPES.get(t.dtype)
+    if kind is None:
         raise TypeError(f"{name} must be bfloat16, float16 or float32, got {t.dtype}")
     if t.dim() != 2 or not 1 <= t.shape[1] <= _MAX_COLUMNS:
         raise ValueError(f"{name} must be a matrix of 1 .. {_MAX_COLUMNS} columns, got shape {tuple(t.shape)}")
-    return _ROW_TYPES[t.dtype]
+    return kind
 
 
 # Tangents of forward-mode differentiation go with tensors that want no gradient.  A result without one would say that it is zero.
@@ -130,15 +131,16 @@ _written = torch._C._increment_version
 def plan_rows(num_tokens: int, top_k: int, num_experts: int, align: int = 1) -> int:
     """Rows that any choice of experts fits into: what `rows` of a dispatch must hold."""
     given = num_tokens, top_k, num_experts, align
-    T, K, E, align = whole = int(num_tokens), int(top_k), int(num_experts), int(align)
-    if whole == given and 0 <= T <= _SMALL and 1 <= K <= _lib.PLAN_MAX_TOP_K and 1 <= E <= _lib.PLAN_MAX_EXPERTS and 1 <= align <= 1024:
-        pairs = T * K
-        return (pairs + min(E, pairs) * (align - 1) + align - 1) // align * align
+    if (type(num_tokens) is type(top_k) is type(num_experts) is type(align) is int and 0 <= num_tokens <= _SMALL
+            and 1 <= top_k <= _lib.PLAN_MAX_TOP_K and 1 <= num_experts <= _lib.PLAN_MAX_EXPERTS and 1 <= align <= 1024):
+        pairs = num_tokens * top_k
+        return (pairs + min(num_experts, pairs) * (align - 1) + align - 1) // align * align
+    whole = int(num_tokens), int(top_k), int(num_experts), int(align)
     # what passes 32 bits would reach the library cut to them
     rows = _lib.load().moe_fp8_b200_plan_rows(*whole) if whole == given and max(whole) < 1 << 31 and min(whole) >= 0 else -1
     if rows < 0:
         raise ValueError(f"no plan for {num_tokens} tokens, top_k {top_k} (1 .. {_lib.PLAN_MAX_TOP_K}), {num_experts} experts "
-                         f"(1 .. {_lib.PLAN_MAX_EXPERTS}), align {given[3]} (1 .. 1024)")
+                         f"(1 .. {_lib.PLAN_MAX_EXPERTS}), align {align} (1 .. 1024)")
     return int(rows)
 
 
@@ -210,9 +212,10 @@ def _check_plan(plan):
 def _ids(topk_idx, num_experts, first_expert, align, plan):
     """The plan to fill for these ids."""
     index = _on_gpu("topk_idx", topk_idx)
-    first_expert = operator.index(first_expert)
-    if not -1 << 63 <= first_expert <= (1 << 63) - max(1, int(num_experts)):   # the library counts on from it modulo 2^64
-        raise ValueError(f"first_expert {first_expert}: experts from it on are not 64-bit ids")
+    if type(first_expert) is not int or not 0 <= first_expert <= _SMALL:
+        # the library counts on from it modulo 2^64
+        if not -1 << 63 <= operator.index(first_expert) <= (1 << 63) - max(1, int(num_experts)):
+            raise ValueError(f"first_expert {first_expert}: experts from it on are not 64-bit ids")
     if topk_idx.dtype not in _ID_BITS:
         raise TypeError(f"topk_idx must be int32 or int64, got {topk_idx.dtype}")
     if topk_idx.dim() != 2:
@@ -350,17 +353,19 @@ def combine_backward(grad_out, y, weights, plan: ExpertPlan, grad_y=None, grad_w
     _check_plan(plan)
     if _forward_ad._current_level >= 0:
         _no_tangents(grad_out=grad_out, y=y, weights=weights)
-    for t in (grad_out, y, weights):
-        if isinstance(t, torch.Tensor) and t.requires_grad and torch.is_grad_enabled():
-            raise ValueError("combine_backward has no gradient: call it under torch.no_grad()")
     kind = _row_type("grad_out", grad_out)
     H, dtype, device, index = grad_out.shape[1], grad_out.dtype, plan._device, plan._index
     gp, gs = _matrix("grad_out", grad_out, plan._num_tokens, H, dtype, index)
     yp, ys, wp, dp, ds, dwp = None, 0, None, None, 0, None
+    wanted = grad_out.requires_grad
     if need_weights or y is not None:
         yp, ys = _matrix("y", y, plan._capacity, H, dtype, index)
+        wanted |= y.requires_grad
     if need_y or weights is not None:
         wp = _packed("weights", weights, torch.float32, (plan._num_tokens, plan._top_k), index)
+        wanted |= weights.requires_grad
+    if wanted and torch.is_grad_enabled():
+        raise ValueError("combine_backward has no gradient: call it under torch.no_grad()")
     fresh = grad_y is None
     if need_y:
         if fresh:
