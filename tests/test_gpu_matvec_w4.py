@@ -437,3 +437,21 @@ def test_a_small_value_under_a_large_one_is_exact(pkg, M, zeros, dtype):
         want[M - 1] = x[M - 1, 40]
         assert bool(want[M - 1].any())
         assert torch.equal(pkg.matvec_w4(x, codes, scales, zeros=z), want), k
+
+
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("zeros", [False, True])
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("M,N,K,group", [(3, 48, 3104, 32), (2, 32, 3104, 32), (9, 32, 4096, 32), (4, 64, 2080, 32), (5, 48, 2112, 64),
+                                         (1, 80, 3968, 128)])
+def test_eight_warps_per_tile(pkg, M, N, K, group, dtype, zeros, gated):
+    """2048 < K <= 4096, with rows that are no multiple of 256 columns and odd numbers of 32-column blocks."""
+    codes, scales, z = make_weights((), N, K, group, dtype, zeros, M + N + K)
+    x = torch.randn(M, K, generator=torch.Generator(device="cuda").manual_seed(1), device="cuda").to(dtype)
+    if gated and zeros and (K // group) % 2:
+        with pytest.raises(pkg.MoeError, match="even number of groups"):
+            pkg.matvec_w4(x, codes, scales, zeros=z, gated=True)
+        return
+    got = pkg.matvec_w4(x, codes, scales, zeros=z, gated=gated)
+    want, bound = expect(x, decoded(codes, scales, z), gated)
+    assert got.shape == want.shape and close(got, want, bound, dtype)
