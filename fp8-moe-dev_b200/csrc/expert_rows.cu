@@ -386,8 +386,12 @@ __global__ void __launch_bounds__(256) dispatch_rows_kernel(Rows x, Rows rows, i
 }
 
 // A small batch sorted and copied by one kernel: every CTA sorts all pairs for itself, one of them writes the plan.  Up to 2048
-// pairs that costs less than a second launch and the wait between the two (top 8, 7168 columns, us by one and by two
-// kernels: 1 token 8.2 / 11.3, 128 tokens 13.2 / 17.4, 256 tokens 16.4 / 19.4, 512 tokens 28.7 / 25.6).
+// pairs that costs less than a second launch and the wait between the two (top 8 of 256 experts, 7168 columns, align 1, given
+// rows, us by one and by two kernels, call by call: 1 token 8.2 / 11.3, 128 tokens 13.2 / 17.4, 256 tokens 16.4 / 19.4, 512 tokens
+// 28.7 / 25.6; replayed in a graph: 3.5 / 4.5, 7.9 / 9.1, 12.1 / 12.1; align 8 in a graph: 7.2 / 7.6, 12.5 / 14.0, 14.8 / 15.2).
+// The rule looks at neither align nor new rows, where it costs more than it gives: the CTAs that write zeros sort as well, and
+// there are thousands of them (in a graph, 1 token and 256 tokens: align 32 40 / 15 and 42 / 31, align 128 41 / 16 and 75 / 79;
+// new rows at align 1 12.9 / 6.7 and 18.1 / 14.1).
 constexpr int kSmallPairs = 2048, kSmallTokens = 256, kSmallThreads = 256;
 
 template <typename Id, typename T, int N>

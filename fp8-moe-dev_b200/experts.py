@@ -6,8 +6,9 @@ the experts' rows back at their tokens with the routing weights applied, and the
     y = ...                                                # the experts' results, row by row
     out = combine(y, topk_weights, plan)                   # [T, hidden]
 
-`sort_and_dispatch` is the first two in one call.  `dispatch` and `combine` take part in autograd; `dispatch_backward`
-and `combine_backward` are their gradients as plain calls.  Results go to the tensors passed for them, or to new ones.
+`sort_and_dispatch` is the first two in one call.  `dispatch` and `combine` take part in autograd, in reverse mode;
+`dispatch_backward` and `combine_backward` are their gradients as plain calls.  Tensors with a tangent of forward mode are refused
+everywhere.  A plan written to after a forward pass is refused by its backward pass.  Results go to the tensors passed for them, or to new ones.
 Everything runs on the current stream of the tensors' device, returns without synchronising and may be captured into a
 graph.  (A captured backward pass follows torch's own rule: no other graph of the same leaves may be alive, since the nodes that
 accumulate their gradients belong to the stream that made them.  The `_backward` functions have no such rule.)  `matvec_w4`
@@ -392,7 +393,7 @@ def combine_backward(grad_out, y, weights, plan: ExpertPlan, grad_y=None, grad_w
 def matvec_w4(x, codes, scales, *, zeros=None, plan: Optional[ExpertPlan] = None, by_token: bool = False, gated: bool = False,
               out=None):
     """Products of a few rows with 4-bit weights: y[r, n] = sum_k (code[n, k] - zero[n, g]) * scale[n, g] * x[r, k] with
-    g = k // group, summed in fp32 and rounded once.
+    g = k // group: exact products of codes and x, summed in fp32, rounded once.
 
       codes   uint8 [E, n, k / 2]          two codes 0 .. 15 per byte, the even column in the low half
       scales  x's dtype [E, n, k / group]  group 32, 64 or 128
@@ -403,7 +404,11 @@ def matvec_w4(x, codes, scales, *, zeros=None, plan: Optional[ExpertPlan] = None
     are those of a single matrix (no E), and x and out have as many rows as x.
     gated: the weights hold n / 2 linear rows, then n / 2 gated ones, and out [.., n / 2] is silu(gated) * linear.
     x is bfloat16 or float16; n a multiple of 16, k of the group and at most 8192.  The weights are read once per eight
-    rows of an expert: for decode batches."""
+    rows of an expert: for decode batches.
+
+    Equal calls give equal bits.  The order of a sum depends on how many rows the expert has, and on the values, so that a row's
+    last bits may differ between batches.  A weight that never arrives (a wait of a second) leaves NaN in the results, and no
+    error.  Not differentiable."""
     index = _on_gpu("x", x)
     kind = _row_type("x", x)
     if kind == _lib.FP32:
