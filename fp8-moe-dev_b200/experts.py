@@ -7,8 +7,9 @@ the experts' rows back at their tokens with the routing weights applied, and the
     out = combine(y, topk_weights, plan)                   # [T, hidden]
 
 `sort_and_dispatch` is the first two in one call.  `dispatch` and `combine` take part in autograd, in reverse mode;
-`dispatch_backward` and `combine_backward` are their gradients as plain calls.  Tensors with a tangent of forward mode are refused
-everywhere.  A plan written to after a forward pass is refused by its backward pass.  Results go to the tensors passed for them, or to new ones.
+`dispatch_backward` and `combine_backward` are their gradients as plain calls.  Tensors with a tangent of forward mode are
+refused everywhere.  A plan written to after a forward pass is refused by its backward pass.  Results go to the tensors passed
+for them, or to new ones.
 Everything runs on the current stream of the tensors' device, returns without synchronising and may be captured into a
 graph.  (A captured backward pass follows torch's own rule: no other graph of the same leaves may be alive, since the nodes that
 accumulate their gradients belong to the stream that made them.  The `_backward` functions have no such rule.)  `matvec_w4`
